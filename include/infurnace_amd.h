@@ -503,6 +503,110 @@ int ifn_copy_pages(void* kv_pool, int32_t num_layers, int64_t num_pages, const i
                    const int32_t* dst_ids, int32_t num_ids, int32_t num_kv_heads, int32_t head_dim,
                    int32_t block_size, void* stream);
 
+/*
+ * ---- 8-bit KV cache -------------------------------------------------------
+ * One layer's cache is two arrays: codes uint8 (e4m3)
+ * [2][num_pages][num_kv_heads][16][head_dim] (K = 0, V = 1; head-major pages) and
+ * scales fp32 [2][num_pages][num_kv_heads].  A block -- the 16 tokens of a page,
+ * one kv head, of K or of V -- has one scale, a power of two (every other value
+ * is undefined behaviour of the numbers, not of memory); a value is code x scale.
+ * Slots, tables, lengths and masks are those of the fp16 pool.  block_size 16,
+ * head_dim 64, 128 or 256 (prefill: 64 or 128); IFN_ERR_UNSUPPORTED otherwise.
+ * K/V rows and queries must be finite.
+ *
+ * Append: as ifn_store_kv, rounding to e4m3.  For the rows x of the call that
+ * fall into one block: need = 2^max(-32, ceil(log2(max |x| / 448))); when one of
+ * them has offset 0 in the page the block starts anew (scale = need, its rows
+ * that are not stored become zero), else its scale becomes max(scale, need) and
+ * its other codes are rounded to a grown scale.  A page is filled from offset 0
+ * up, so rows behind the stored ones are zero.  The tokens of one page must lie
+ * within 64 consecutive entries of slot_mapping (any order; of two active entries
+ * with one slot the later is stored): a token farther than that from the first of
+ * its page may be dropped or race with it.
+ * Replaces: store_kv, docs/architecture.md:245 (placeholder
+ * src/infurnace/kernels/kv_store.py, 0 B), for a cache of half the bytes; the
+ * reference stores fp16 only.
+ */
+int ifn_store_kv_fp8(void* codes_layer, float* scales_layer, int64_t num_pages,
+                     const int32_t* slot_mapping, const uint8_t* active_mask, const void* new_k,
+                     const void* new_v, int32_t num_tokens, int32_t num_kv_heads, int32_t head_dim,
+                     int32_t block_size, void* stream);
+
+/* Workspace bytes of the two decode calls below (page_weights: non-zero when they gather weights). */
+size_t ifn_paged_decode_fp8_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
+                                            int32_t head_dim, int32_t block_size, int32_t max_pages_per_seq,
+                                            int32_t max_seq_len, int32_t page_weights);
+
+/*
+ * ifn_paged_decode over the 8-bit cache: the attention over the fp16 values
+ * code x scale (exact for blocks written by the append above), fp32
+ * accumulation, probabilities rounded to fp16.  num_q_heads / num_kv_heads up
+ * to 16.  Same rules for rows, lengths, page ids and the workspace.
+ * page_weights (may be NULL): fp32 [batch][num_kv_heads][max_pages_per_seq]; to
+ * entry (b, h, j) is added the sum, over the query heads of kv head h and the
+ * keys of the row's page j, of the attention probabilities.  Entries past a
+ * row's pages, and of inactive rows, are left as they are.
+ * Replaces: paged_attention (decode), docs/architecture.md:246 (placeholder
+ * src/infurnace/kernels/paged_attention.py, 0 B).
+ */
+int ifn_paged_decode_fp8(void* out, const void* query, const void* codes_layer, const float* scales_layer,
+                         int64_t num_pages, const int32_t* block_tables, int32_t max_pages_per_seq,
+                         const int32_t* seq_lens, const uint8_t* active_mask, float* page_weights,
+                         int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                         int32_t block_size, int32_t max_seq_len, float scale, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/*
+ * The decode step's append and attention in one launch: new_k / new_v
+ * [batch][num_kv_heads][head_dim] fp16 are stored at position seq_lens[b] - 1 of
+ * row b's table, as ifn_store_kv_fp8 stores them, then the row attends over its
+ * seq_lens[b] tokens.  Rows that are inactive, empty, longer than max_seq_len or
+ * whose last page id is outside the pool store nothing.  Precondition: a row's
+ * last page is in no other row's table.
+ * Replaces: store_kv then paged_attention of a decode step
+ * (docs/architecture.md:245-246).
+ */
+int ifn_paged_decode_append_fp8(void* out, const void* query, void* codes_layer, float* scales_layer,
+                                int64_t num_pages, const int32_t* block_tables, int32_t max_pages_per_seq,
+                                const int32_t* seq_lens, const uint8_t* active_mask, const void* new_k,
+                                const void* new_v, float* page_weights, int32_t batch, int32_t num_q_heads,
+                                int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                                int32_t max_seq_len, float scale, void* workspace, size_t workspace_bytes,
+                                void* stream);
+
+/*
+ * ifn_paged_prefill over the 8-bit cache (the chunk's K/V stored before it).
+ * Any group size; no workspace.
+ * Replaces: paged_attention with a multi-token query, docs/architecture.md:246.
+ */
+int ifn_paged_prefill_fp8(void* out, const void* query, const void* codes_layer, const float* scales_layer,
+                          int64_t num_pages, const int32_t* block_table, int32_t max_pages,
+                          int32_t query_start, int32_t num_q_tokens, int32_t num_q_heads,
+                          int32_t num_kv_heads, int32_t head_dim, int32_t block_size, float scale,
+                          void* stream);
+
+/*
+ * Eviction by accumulated attention weight: row b of n = ceil(seq_lens[b] / 16)
+ * pages with n > keep_pages keeps its first sink_pages and last recent_pages and,
+ * of the others, the keep_pages - sink_pages - recent_pages of largest weight
+ * (page_weights summed over kv heads in 64 bits and rounded to fp32; NaN lowest,
+ * ties to the lower index).  out_tables: the kept ids in order, then the evicted
+ * ones in order, then the entries past the row's pages as they were.
+ * out_weights: the kept pages' weights in the same order, zeros after them.
+ * out_lens = seq_lens - 16 x evicted; num_evicted[b] counts the evicted pages.
+ * Other rows (and inactive ones) are copied, their weights past n zeroed.  The
+ * outputs must not overlap the inputs.  recent_pages >= 1 (the last page may be
+ * partial), keep_pages >= sink_pages + recent_pages; max_pages_per_seq up to
+ * 32768 (IFN_ERR_UNSUPPORTED).  Lengths are clamped to the table for n.
+ * Replaces: nothing in the reference, whose cache rows only grow; it works on
+ * the tables of docs/architecture.md:234-240.
+ */
+int ifn_evict_pages(int32_t* out_tables, int32_t* out_lens, float* out_weights, int32_t* num_evicted,
+                    const int32_t* block_tables, int32_t max_pages_per_seq, const int32_t* seq_lens,
+                    const uint8_t* active_mask, const float* page_weights, int32_t batch,
+                    int32_t num_kv_heads, int32_t block_size, int32_t keep_pages, int32_t sink_pages,
+                    int32_t recent_pages, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
