@@ -15,6 +15,7 @@
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -38,7 +39,10 @@ namespace {
   X(prefill_ws, ifn_paged_prefill_workspace_bytes) X(prefill, ifn_paged_prefill) \
   X(prefill_append, ifn_paged_prefill_append) X(prep_append, ifn_qk_norm_rope_append) \
   X(prep_decode, ifn_paged_decode_prep_append) X(prep_decode_planning, ifn_paged_decode_prep_append_planning) \
-  X(prep_prefill, ifn_paged_prefill_prep_append)
+  X(prep_prefill, ifn_paged_prefill_prep_append) X(store_fp8, ifn_store_kv_fp8) \
+  X(decode_fp8_ws, ifn_paged_decode_fp8_workspace_bytes) X(decode_fp8, ifn_paged_decode_fp8) \
+  X(decode_append_fp8, ifn_paged_decode_append_fp8) X(prefill_fp8, ifn_paged_prefill_fp8) \
+  X(evict_pages, ifn_evict_pages)
 struct Entries {
 #define IFN_MEMBER(name, fn) decltype(&fn) name;
   IFN_ENTRIES(IFN_MEMBER)
@@ -514,6 +518,133 @@ PyObject* store_layers(PyObject* const* a) {
   Py_RETURN_TRUE;
 }
 
+// One layer of the 8-bit cache (kv_fp8._check_cache).  The calls that follow are made on the current device only, and
+// not under graph capture (where the Python path gives a call a workspace of its own).
+struct Cache : Pool {
+  float* scales;
+};
+
+Cache cache8(PyObject* kv, PyObject* sc, int64_t layer) {
+  const at::Tensor& t = tensor(kv, at::kFloat8_e4m3fn);
+  need(t.dim() == 5 || t.dim() == 6);
+  const int64_t k = t.dim() - 5;  // dims before [2, P, Hkv, 16, D]
+  const at::Tensor& s = tensor(sc, at::kFloat, t.get_device());
+  need(s.dim() == t.dim() - 2);
+  for (int64_t i = 0; i < t.dim(); ++i) need(t.size(i) >= 1 && (i >= s.dim() || s.size(i) == t.size(i)));
+  need(t.size(k) == 2 && t.size(k + 3) == 16 && layer >= 0 && layer < (k == 1 ? t.size(0) : 1));
+  Cache r;
+  r.layers = k == 1 ? t.size(0) : 1;
+  r.pages = t.size(k + 1);
+  r.hkv = small(t.size(k + 2));
+  r.bs = 16;
+  r.d = small(t.size(k + 4));
+  r.dev = t.get_device();
+  need(r.dev == c10::hip::current_device());
+  r.p = static_cast<char*>(t.data_ptr()) + layer * 2 * r.pages * r.hkv * 16 * r.d;
+  r.scales = static_cast<float*>(s.data_ptr()) + layer * 2 * r.pages * r.hkv;
+  return r;
+}
+
+bool capturing(void* stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  return hipStreamIsCapturing(static_cast<hipStream_t>(stream), &status) != hipSuccess ||
+         status != hipStreamCaptureStatusNone;
+}
+
+// store_fp8(kv_pool, scales, slot_mapping, active_mask, new_k, new_v, layer)
+PyObject* store_fp8(PyObject* const* a) {
+  const Cache P = cache8(a[0], a[1], integer(a[6]));
+  const at::Tensor& k = tensor(a[4], at::kHalf, P.dev);
+  need(k.dim() == 3 && k.size(0) >= 1);
+  const int64_t n = k.size(0);
+  shaped(a[4], at::kHalf, P.dev, n, P.hkv, P.d);
+  const at::Tensor& v = shaped(a[5], at::kHalf, P.dev, n, P.hkv, P.d);
+  launched(launch(E.store_fp8, P.p, P.scales, P.pages, i32(a[2], P.dev, n), mask(a[3], P.dev, n), k.data_ptr(),
+                  v.data_ptr(), small(n), P.hkv, P.d, P.bs, stream_of(P.dev)), "ifn_store_kv_fp8");
+  Py_RETURN_TRUE;
+}
+
+// decode_fp8(query, kv_pool, scales, block_tables, sequence_lengths, active_mask, new_k, new_v, layer, scale, out,
+//            max_seq_len, page_weights, workspaces); new_k None: attention alone
+PyObject* decode_fp8(PyObject* const* a) {
+  const Cache P = cache8(a[1], a[2], integer(a[8]));
+  const at::Tensor& q = tensor(a[0], at::kHalf, P.dev);
+  need(q.dim() == 3 && q.size(2) == P.d && q.size(1) % P.hkv == 0 && q.size(0) >= 1 && q.size(1) >= 1);
+  const int64_t n = q.size(0), hq = q.size(1);
+  const at::Tensor& bt = tensor(a[3], at::kInt, P.dev);
+  need(bt.dim() == 2 && bt.size(0) == n && bt.size(1) >= 1);
+  const int32_t* sl = i32(a[4], P.dev, n);
+  const uint8_t* act = mask(a[5], P.dev, n);
+  const bool append = a[6] != Py_None;
+  const void* nk = append ? shaped(a[6], at::kHalf, P.dev, n, P.hkv, P.d).data_ptr() : nullptr;
+  const void* nv = append ? shaped(a[7], at::kHalf, P.dev, n, P.hkv, P.d).data_ptr() : nullptr;
+  const float scale = scale_of(a[9], P.d);
+  const int32_t msl = small(cap_of(a[11], bt.size(1) * P.bs)), B = small(n), Q = small(hq), mp = small(bt.size(1));
+  float* pw = a[12] == Py_None ? nullptr
+                               : static_cast<float*>(shaped(a[12], at::kFloat, P.dev, n, P.hkv, bt.size(1)).data_ptr());
+  const Call c = call_on(a[13], P.dev, E.decode_fp8_ws(B, Q, P.hkv, P.d, P.bs, mp, msl, pw != nullptr));
+  need(!capturing(c.stream));
+  const at::Tensor out = output(a[10], P, n, hq, act != nullptr);
+  const int32_t* tab = static_cast<const int32_t*>(bt.data_ptr());
+  void* o = out.data_ptr();
+  const void* qp = q.data_ptr();
+  const int rc = append ? launch(E.decode_append_fp8, o, qp, P.p, P.scales, P.pages, tab, mp, sl, act, nk, nv, pw, B, Q,
+                                 P.hkv, P.d, P.bs, msl, scale, c.ws, c.bytes, c.stream)
+                        : launch(E.decode_fp8, o, qp, P.p, P.scales, P.pages, tab, mp, sl, act, pw, B, Q, P.hkv, P.d,
+                                 P.bs, msl, scale, c.ws, c.bytes, c.stream);
+  launched(rc, append ? "ifn_paged_decode_append_fp8" : "ifn_paged_decode_fp8");
+  return done(out, a[10]);
+}
+
+// prefill_fp8(query, kv_pool, scales, block_table, query_start, layer, scale, out)
+PyObject* prefill_fp8(PyObject* const* a) {
+  const Cache P = cache8(a[1], a[2], integer(a[5]));
+  const at::Tensor& q = tensor(a[0], at::kHalf, P.dev);
+  need(q.dim() == 3 && q.size(2) == P.d && q.size(1) % P.hkv == 0 && q.size(0) >= 1 && q.size(1) >= 1);
+  const int64_t n = q.size(0), hq = q.size(1), start = integer(a[4]);
+  int64_t mp;
+  const at::Tensor& bt = table_of(a[3], P.dev, mp);
+  need(start >= 0 && start + n <= mp * P.bs);
+  const float scale = scale_of(a[6], P.d);
+  const at::Tensor out = output(a[7], P, n, hq, false);
+  launched(launch(E.prefill_fp8, out.data_ptr(), q.data_ptr(), P.p, P.scales, P.pages,
+                  static_cast<const int32_t*>(bt.data_ptr()), small(mp), int32_t(start), small(n), small(hq), P.hkv, P.d,
+                  P.bs, scale, stream_of(P.dev)), "ifn_paged_prefill_fp8");
+  return done(out, a[7]);
+}
+
+// evict(block_tables, sequence_lengths, page_weights, keep_pages, sink_pages, recent_pages, active_mask, block_size)
+PyObject* evict(PyObject* const* a) {
+  const at::Tensor& bt = tensor(a[0], at::kInt);
+  const int dev = bt.get_device();
+  need(bt.dim() == 2 && bt.size(0) >= 1 && bt.size(1) >= 1 && dev == c10::hip::current_device());
+  const int64_t n = bt.size(0), mp = bt.size(1);
+  const int32_t* sl = i32(a[1], dev, n);
+  const at::Tensor& w = tensor(a[2], at::kFloat, dev);
+  need(w.dim() == 3 && w.size(0) == n && w.size(1) >= 1 && w.size(2) == mp);
+  int64_t keep = integer(a[3]), sink = integer(a[4]), recent = integer(a[5]);
+  need(sink >= 0 && recent >= 1 && keep >= sink + recent);
+  if (keep >= mp) {  // no row holds more
+    keep = mp;
+    sink = 0;
+    recent = 1;
+  }
+  const uint8_t* act = mask(a[6], dev, n);
+  const int32_t bs = small(integer(a[7]));
+  at::Tensor t, l, ow, g;
+  unlocked([&] { t = at::empty({n, mp}, bt.options()); l = at::empty({n}, bt.options()); ow = at::empty({n, w.size(1), mp}, w.options()); g = at::empty({n}, bt.options()); });
+  launched(launch(E.evict_pages, static_cast<int32_t*>(t.data_ptr()), static_cast<int32_t*>(l.data_ptr()),
+                  static_cast<float*>(ow.data_ptr()), static_cast<int32_t*>(g.data_ptr()),
+                  static_cast<const int32_t*>(bt.data_ptr()), small(mp), sl, act, static_cast<const float*>(w.data_ptr()),
+                  small(n), small(w.size(1)), bs, int32_t(keep), int32_t(sink), int32_t(recent), stream_of(dev)),
+           "ifn_evict_pages");
+  PyObject* r = PyTuple_New(4);
+  need(r != nullptr);
+  const at::Tensor* all[] = {&t, &l, &ow, &g};
+  for (int i = 0; i < 4; ++i) PyTuple_SET_ITEM(r, i, THPVariable_Wrap(*all[i]));
+  return r;
+}
+
 // A call of N arguments: None when it is not one for this path (no C++ exception leaves it).
 template <PyObject* (*F)(PyObject* const*), Py_ssize_t N>
 PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -586,6 +717,7 @@ PyObject* bind(PyObject*, PyObject* args) {
 PyMethodDef methods[] = {
     IFN_FAST(decode, 16), IFN_FAST(prep_decode, 20), IFN_FAST(prefill, 11), IFN_FAST(prep_prefill, 15),
     IFN_FAST(prep_append, 13), IFN_FAST(store, 6), IFN_FAST(store_layers, 5),
+    IFN_FAST(store_fp8, 7), IFN_FAST(decode_fp8, 14), IFN_FAST(prefill_fp8, 8), IFN_FAST(evict, 8),
     {"bind", bind, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast_call", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

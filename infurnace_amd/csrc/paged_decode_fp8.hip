@@ -5,26 +5,29 @@
 // contiguous semantics src/infurnace/executor/tinygrad/model.py:196-200): out = softmax(scale q K^T) V over the
 // row's first L tokens, query head h reading kv head h / G.  Blocks and scales: kv_fp8.hpp.
 //
-//  * A wave attends one kv head.  The pages of all rows, row after row, form one list per head; the grid's
-//    waves are Hkv x (streams), and stream r takes pages [T r / nr, T (r+1) / nr) of the list for its head, so
-//    ragged batches cost every wave the same bytes.  Waves share nothing but the rows' offsets in the list
-//    (LDS); Hkv and the group size G (up to 16) are run-time numbers.  A row that starts inside a range costs
-//    it kRowStart pages more (its query, its first loads).
-//  * Two pages (32 tokens) are one step: S^T = K Q^T and O^T += V^T P^T with v_mfma_f32_16x16x32_f16, the
-//    group's queries in the 16 columns.  Lane (n = lane % 16, g = lane / 16) loads K of token n, dims
-//    64 i + 16 g .. + 15 (the fragments' k order is theirs to choose, as long as Q's is the same), gets the
-//    scores of query n and tokens 4 g .. 4 g + 3 of each page, and needs V of the same tokens for the second
-//    product: it loads 4 token rows x D / 16 dims of V and transposes the bytes (v_perm).  So codes go from
-//    memory to the matrix cores without LDS and without an exchange between lanes; only the running maximum
-//    is reduced over the four g (v_permlane swaps).  The running sum stays a lane's own until the end.
+//  * A wave attends one kv head.  The pages of all rows, row after row, form one list per head, which the grid's
+//    waves cut into ranges: stream r takes pages [T r / nr, T (r+1) / nr), so ragged batches cost every wave the
+//    same bytes.  Hkv and the group size G (up to 16) are run-time numbers.
+//  * S^T = K Q^T with v_mfma_f32_16x16x32_f16 and O^T += V^T P^T with v_mfma_f32_16x16x16_f16, the group's queries in
+//    the 16 columns, a page's tokens in the 16 rows.  Lane (n = lane % 16, g = lane / 16) loads K of token n, dims
+//    64 i + 16 g .. + 15 (the fragments' k order is theirs to choose, as long as Q's is the same), gets the scores of
+//    query n and tokens 4 g .. 4 g + 3, and needs V of the same tokens for the second product: it loads 4 token rows
+//    x D / 16 dims of V and transposes the bytes (v_perm).  So codes go from memory to the matrix cores without LDS
+//    and without an exchange between lanes; only the running maximum is reduced over the four g (v_permlane swaps).
+//    The running sum stays a lane's own until the end.
 //  * Codes become fp16 exactly (kv_fp8.hpp).  Probabilities are rounded to fp16 for the second product (2^-12
 //    relative, averaged over the keys); scores, maxima, sums and outputs are fp32.
-//  * A row held by several streams: their states (m, l, O in fp32) go to the workspace and the wave that
-//    arrives last, by a ticket per (row, head), merges them in range order.
+//  * A row held by several ranges: the four waves of a workgroup have consecutive ranges of one head and merge their
+//    states (m, l, O in fp32) in LDS; what other workgroups hold too goes to the workspace, and the workgroup that
+//    arrives last, by a ticket per (row, head), merges it in range order.
 //  * Fused append (kAppend): the wave that holds a row's last page adds the row's new token to the block in
 //    its registers (new scale, rescaled codes), stores what changed and attends over the result.
-//  * Page weights (kWeights): each page's log2-sum-exp per query head goes to the workspace; the wave that
-//    finishes a (row, head) turns them into sum_g exp2(lse - total) and adds them to page_weights.
+//  * Page weights (kWeights): each page's log2-sum-exp per query head goes to the workspace; whoever finishes a
+//    (row, head) turns them into sum_g exp2(lse - total) and adds them to page_weights.
+//
+// What bounds it: memory, above about 100 MB.  128 rows of 1023-8190 keys, 32 / 8 heads x 128 (1.21 GB): 213 us, 5.7
+// TB/s; 32 rows of 128-4096, 16 / 8 heads (143 MB): 34 us, of which about 4 before a wave's first page (lengths, ids,
+// scales), 20 streaming, 3 of uneven waves and 7 after (states written through to memory, ticket, merge).
 #include <algorithm>
 #include <type_traits>
 
@@ -32,12 +35,24 @@
 
 namespace ifn {
 
-constexpr int kF8DecThreads = 512;
-constexpr int kF8DecWaves = kF8DecThreads / kWave;
+// Threads of a workgroup.  Small ones: a workgroup's waves wait for each other before they merge (one row of 512
+// keys 10.2 us with 256, 12.6 with 512; 48 rows of 100-4000, 2 kv heads, 23.3 and 29.4).
+constexpr int kDecThreads = 256;
+constexpr int kDecWaves = kDecThreads / kWave;
+constexpr int kDecPerSimd = 2;     // waves a SIMD is to hold (registers)
+constexpr int f8_per_simd(int d) { return d == 256 ? 1 : kDecPerSimd; }
+// Pages in a wave's ring.  The memory is as busy with 2 as with 4 (128 rows of 1023-8190 keys: 213 and 214 us), and
+// short pieces request fewer pages twice (32 rows of 128-4096: 35.2 and 37.1 us).
+constexpr int kRing = 2;
 constexpr int kF8MaxBatch = 4096;  // rows per call (LDS offsets)
 constexpr int kF8MaxGroup = 16;    // query heads per kv head (MFMA columns)
-constexpr int kRowStart = 1;       // pages a row's start counts for in the split
+// Pages a row's start counts for in the split: its ids, scales and query take three round trips before the first
+// page (32 rows of 128-4096 keys: 37.1, 36.8 and 36.0 us with 1, 2 and 3; 64 rows of 256 dims 58.1, 56.3, 55.1).
+constexpr int kRowStart = 3;
 constexpr int kMinPages = 2;       // fewest list positions per range
+// Most ranges per row of the call.  A row's states are merged 16 workgroups a round trip, so more than 64 waves a row
+// cost another one (one row of 8000 keys, 32 / 8 heads: 17.9, 14.8, 15.6 and 20.4 us with 32, 64, 128 and 250 ranges).
+constexpr int kMaxRanges = 64;
 
 struct F8Cache {
   uint8_t* codes;
@@ -49,7 +64,7 @@ struct F8Append {
   const f16* new_v;
 };
 // Workspace: [tickets][ml: slots x Hkv x G x 2][o: slots x Hkv x G x D][lse: batch x Hkv x max_pages x G], fp32;
-// slot = row + range.
+// slot = row + workgroup (of a head).
 struct F8Workspace {
   uint32_t* count;
   float* ml;
@@ -80,8 +95,12 @@ __device__ __forceinline__ float swap_sum(float x) {  // over lanes l, l ^ 16, l
 __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
+__device__ __forceinline__ f32x4 mfma16(f16x4 a, f16x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0);
+}
 #else
 __device__ __forceinline__ f32x4 mfma16(f16x8, f16x8, f32x4 c) { return c; }
+__device__ __forceinline__ f32x4 mfma16(f16x4, f16x4, f32x4 c) { return c; }
 #endif
 
 // One page of one head as loaded: K chunk i = 16 dims of token n, V row t = D / 16 dims of token 4 g + t.
@@ -93,11 +112,21 @@ struct F8Page {
 };
 
 // Pages of row b in the list: its own, and kRowStart more in front when it has any.
+// No instruction: the values must have arrived at this point.
+template <class A, class B>
+__device__ __forceinline__ void settle(A& a, B& b) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" : "+v"(a));
+  asm volatile("" : "+v"(b));
+#endif
+}
+
+template <int kWaves>
 __device__ __forceinline__ int f8_offsets(int* s_cum, int* s_wsum, const int32_t* seq_lens, const uint8_t* active,
                                           int batch, int cap) {
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   int running = 0;
-  for (int base = 0; base < batch; base += kF8DecThreads) {
+  for (int base = 0; base < batch; base += kWaves * kWave) {
     const int i = base + tid;
     int n = 0;
     if (i < batch) {
@@ -116,7 +145,7 @@ __device__ __forceinline__ int f8_offsets(int* s_cum, int* s_wsum, const int32_t
     if (lane == kWave - 1) s_wsum[wave] = x;
     __syncthreads();
     int pre = 0, tot = 0;
-    for (int w = 0; w < kF8DecWaves; ++w) {
+    for (int w = 0; w < kWaves; ++w) {
       const int v = s_wsum[w];
       pre += w < wave ? v : 0;
       tot += v;
@@ -130,8 +159,48 @@ __device__ __forceinline__ int f8_offsets(int* s_cum, int* s_wsum, const int32_t
   return running;
 }
 
+// The end of a row split over ranges: its np states, slots slot0 + j hkv, merged in range order for the 4-dim unit u
+// of query un (kMergeBatch states a round trip).
+constexpr int kMergeBatch = 16;
+__device__ __forceinline__ void f8_merge(__amdgpu_buffer_rsrc_t r_ml, __amdgpu_buffer_rsrc_t r_o, int64_t slot0, int hkv,
+                                         int np, int G, int D, int un, int u, float& M, float& L, f32x4& O) {
+  M = kNegBig;
+  L = 0.f;
+  O = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int j0 = 0; j0 < np; j0 += kMergeBatch) {
+    const int cnt = min(kMergeBatch, np - j0);
+    f32x2 ml[kMergeBatch];
+    f32x4 o[kMergeBatch];
+#pragma unroll
+    for (int x = 0; x < kMergeBatch; ++x) {
+      if (x < cnt) {
+        const uint32_t sl = uint32_t(slot0 + int64_t(j0 + x) * hkv);
+        ml[x] = ld_dev2(r_ml, (sl * G + un) * 8);
+        o[x] = ld_dev4(r_o, (sl * G * D + u * 4) * 4);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    float gm = M;
+#pragma unroll
+    for (int x = 0; x < kMergeBatch; ++x)
+      if (x < cnt) gm = fmaxf(gm, ml[x][0]);
+    const float sc = exp2_fast(M - gm);
+    M = gm;
+    L *= sc;
+    O = f32x4{O[0] * sc, O[1] * sc, O[2] * sc, O[3] * sc};
+#pragma unroll
+    for (int x = 0; x < kMergeBatch; ++x) {
+      if (x < cnt) {
+        const float w = exp2_fast(ml[x][0] - M);
+        L = fmaf(w, ml[x][1], L);
+        O = f32x4{fmaf(w, o[x][0], O[0]), fmaf(w, o[x][1], O[1]), fmaf(w, o[x][2], O[2]), fmaf(w, o[x][3], O[3])};
+      }
+    }
+  }
+}
+
 template <int D, bool kAppend, bool kWeights>
-__global__ __launch_bounds__(kF8DecThreads) void decode_fp8_kernel(
+__global__ __launch_bounds__(kDecThreads, f8_per_simd(D)) void decode_fp8_kernel(
     f16* __restrict__ out, const f16* __restrict__ q, F8Cache cache, const int32_t* __restrict__ block_tables,
     int32_t max_pages, const int32_t* __restrict__ seq_lens, const uint8_t* __restrict__ active, int32_t batch,
     int32_t hkv, int32_t G, int32_t max_len, float scale_log2, F8Workspace ws, F8Append ap,
@@ -139,64 +208,108 @@ __global__ __launch_bounds__(kF8DecThreads) void decode_fp8_kernel(
   constexpr int kKL = F8Page<D>::kKL, kVW = F8Page<D>::kVW;
   constexpr int kT = D / 16;   // output tiles (dims m D / 16 + tile)
   constexpr int kU = D / 16;   // 4-dim units of a lane's outputs: unit r (D / 64) + q = dims of row 4 g + r, 4 q ..
-  __shared__ int s_cum[kF8MaxBatch + 1];
-  __shared__ int s_wsum[kF8DecWaves];
+  constexpr int kWaves = kDecWaves;
+  constexpr int S = kRing;
+  static_assert(kWave % S == 0, "windows are whole turns of the ring");
+  constexpr int kEnt = 2 * kWaves;  // states a workgroup has at its end: at most two a wave
+  __shared__ int s_wsum[kWaves];
+  __shared__ int s_row[kEnt], s_first[kEnt], s_last[kEnt];
+  __shared__ float s_m[kEnt][kF8MaxGroup], s_l[kEnt][kF8MaxGroup], s_tot[kF8MaxGroup];
+  __shared__ uint32_t s_ticket[2];
+  extern __shared__ __attribute__((aligned(16))) f32x4 s_o[];  // [kEnt][G D / 4], then the rows' offsets [batch + 1]
+  int* const s_cum = reinterpret_cast<int*>(s_o + kEnt * G * (D / 4));
   const int lane = threadIdx.x % kWave;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  // kWeights, behind them: a wave's page sums of one window, [kWaves][64][G]
+  float* const my_lse = reinterpret_cast<float*>(s_cum + batch + 1) + wv * kWave * G;
   const int n = lane % 16, g = lane / 16;
   const int cap = min(max_pages * kF8Page, max_len);
-  const int T = f8_offsets(s_cum, s_wsum, seq_lens, active, batch, cap);
+  const int T = f8_offsets<kWaves>(s_cum, s_wsum, seq_lens, active, batch, cap);
 
-  const int64_t wave = int64_t(blockIdx.x) * kF8DecWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int stream = int(wave / hkv), h = int(wave % hkv);
+  const int h = int(blockIdx.x) % hkv, wg = int(blockIdx.x) / hkv;
+  const int stream = wg * kWaves + wv;
   const int hq = hkv * G;
 
   // Active rows without keys get zeros: row b by wave b, b + waves, ... of the grid.
-  for (int64_t b = wave; b < batch; b += int64_t(gridDim.x) * kF8DecWaves) {
+  for (int64_t b = int64_t(blockIdx.x) * kWaves + wv; b < batch; b += int64_t(gridDim.x) * kWaves) {
     if (s_cum[b + 1] == s_cum[b] && (active == nullptr || active[b] != 0)) {
       for (int i = lane; i < hq * D / 8; i += kWave) st16(out + b * hq * D + i * 8, u32x4{0u, 0u, 0u, 0u});
     }
   }
-  const int nr = min(streams, (T + kMinPages - 1) / kMinPages);
-  if (stream >= nr) return;
-  const int t0 = int(int64_t(T) * stream / nr), t1 = int(int64_t(T) * (stream + 1) / nr);
+  const int nr = min(min(streams, kMaxRanges * batch), (T + kMinPages - 1) / kMinPages);
+  if (wg * kWaves >= nr) return;
+  const bool works = stream < nr;  // (the workgroup's last waves may have no range)
+  const int t0 = works ? int(int64_t(T) * stream / nr) : T, t1 = works ? int(int64_t(T) * (stream + 1) / nr) : T;
   auto range_of = [&](int t) -> int { return int((int64_t(t + 1) * nr - 1) / T); };
 
   const int64_t v_codes = cache.num_pages * hkv * (kF8Page * D), v_scales = cache.num_pages * hkv;
   const uint32_t k_lane = n * D + 16 * g, v_lane = 4 * g * D + n * (D / 16);
+  const int units = kU * 4 * G;  // 4-dim units of a state: (x kVW + c) 4 G + g G + n
+  const uint32_t n_states = uint32_t(batch + streams / kWaves) * hkv * G;
+  const __amdgpu_buffer_rsrc_t r_ml = make_rsrc(ws.ml, n_states * 8u), r_o = make_rsrc(ws.o, n_states * D * 4u);
 
   int lo = 0, hi = batch - 1;  // the last row that starts at or before t0
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (s_cum[mid] <= t0) lo = mid; else hi = mid - 1;
   }
-  int npend = 0, pend_b[2] = {0, 0}, pend_f[2] = {0, 0}, pend_np[2] = {0, 0};
+  int npend = 0;  // this wave's states of rows that other ranges hold too: the range's first and last piece, at most
+  if (lane < 2) s_row[2 * wv + lane] = -1;
 
-  // sum_g exp2(lse - total) of every page of (b, h), added to page_weights.  lse_n: lane n's (n < G) total.
-  auto add_weights = [&](int b, float lse_n, int npages) {
+  // sum_g exp2(lse - total) of every page of (b, h), added to page_weights by `threads` threads, the id-th of them here.
+  auto add_weights = [&](int b, auto total, int npages, int id, int threads) __attribute__((always_inline)) {
     const int64_t seg = int64_t(b) * hkv + h;
-    const float* pl = ws.lse + seg * max_pages * G;
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(ws.lse + seg * max_pages * G, uint32_t(npages) * G * 4u);
     float* dst = page_weights + seg * max_pages;
-    for (int j0 = 0; j0 < npages; j0 += kWave) {
-      const int j = j0 + lane;
-      float w = 0.f;
-      for (int x = 0; x < G; ++x) {
-        const float tot = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, lse_n), x));
-        if (j < npages) w += exp2_fast(ld_dev(pl + int64_t(j) * G + x) - tot);
+    constexpr int kB = 4;  // pages a thread has in flight
+    for (int j0 = 0; j0 < npages; j0 += kB * threads) {
+      float w[kB];
+#pragma unroll
+      for (int c = 0; c < kB; ++c) {
+        const int j = j0 + c * threads + id;
+        w[c] = j < npages ? dst[j] : 0.f;
       }
-      if (j < npages) dst[j] += w;
+      for (int x = 0; x < G; x += 4) {  // (the words past a page's group are not used)
+        f32x4 v[kB];
+#pragma unroll
+        for (int c = 0; c < kB; ++c) v[c] = ld_dev4(r, uint32_t((j0 + c * threads + id) * G + x) * 4u);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const float tot = total(min(x + y, G - 1));
+          if (x + y < G) {
+#pragma unroll
+            for (int c = 0; c < kB; ++c) w[c] += exp2_fast(v[c][y] - tot);
+          }
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < kB; ++c) {
+        const int j = j0 + c * threads + id;
+        if (j < npages) dst[j] = w[c];
+      }
     }
   };
 
-  for (int b = lo; b < batch; ++b) {  // pieces of the range
+  for (int b = lo; b < batch && works; ++b) {  // pieces of the range
     const int cb = __builtin_amdgcn_readfirstlane(s_cum[b]) + kRowStart;
     const int npages = __builtin_amdgcn_readfirstlane(s_cum[b + 1]) - cb;
     if (npages <= 0) continue;
     if (cb >= t1) break;
     const int a = max(t0, cb) - cb, e = min(t1, cb + npages) - cb;
     if (a >= e) continue;
-    const int first = range_of(cb), nranges = range_of(cb + npages - 1) - first + 1;
+    const int32_t* bt = block_tables + int64_t(b) * max_pages + a;
+    const int np = e - a;  // the piece's pages, counted from 0 below
+
+    // page ids and scales, one per lane: the window of 64 pages that is being attended and the next one
+    auto load_ids = [&](int w) {
+      const int id = bt[min(w * kWave + lane, np - 1)];
+      return id;
+    };
+    auto in_pool = [&](int id) { return id >= 0 && int64_t(id) < cache.num_pages; };
+    auto load_scale = [&](int id, int64_t half) { return cache.scales[half + int64_t(in_pool(id) ? id : 0) * hkv + h]; };
+    int win = 0;
+    int ids0 = load_ids(0), ids1 = load_ids(1);
     const int row_len = seq_lens[b], len = min(row_len, cap);
-    const int32_t* bt = block_tables + int64_t(b) * max_pages;
 
     // queries: column n holds head h G + n (columns from G on: zeros), in K's order of dims
     f16x8 qf[2 * kKL];
@@ -210,22 +323,36 @@ __global__ __launch_bounds__(kF8DecThreads) void decode_fp8_kernel(
         qf[2 * i + 1] = as_h8(n < G ? x1 : z);
       }
     }
-    // page ids and scales, 64 per window, one per lane
-    int ids = 0, win = a;
-    float ksc = 0.f, vsc = 0.f;
-    auto load_window = [&](int w0) {
-      win = w0;
-      const int id = bt[min(w0 + lane, e - 1)];
-      const bool ok = id >= 0 && int64_t(id) < cache.num_pages;
-      ids = ok ? id : -1;
-      const int64_t at = int64_t(ok ? id : 0) * hkv + h;
-      ksc = cache.scales[at];
-      vsc = cache.scales[v_scales + at];
-    };
-    load_window(a);
+    // the step's token, when its page is in this piece: K dims as a lane's of K, V dims as of V
+    const bool appends = kAppend && e == npages && row_len <= cap;
+    f16x8 xk[kAppend ? 2 * kKL : 1];
+    f16x4 xv[kAppend ? kVW : 1];
+    if constexpr (kAppend) {
+      if (appends) {
+        const f16* nk = ap.new_k + (int64_t(b) * hkv + h) * D + 16 * g;
+        const f16* nv = ap.new_v + (int64_t(b) * hkv + h) * D + n * (D / 16);
+#pragma unroll
+        for (int i = 0; i < kKL; ++i) {
+          xk[2 * i] = as_h8(ld16(nk + 64 * i));
+          xk[2 * i + 1] = as_h8(ld16(nk + 64 * i + 8));
+        }
+#pragma unroll
+        for (int j = 0; j < kVW; ++j) xv[j] = *reinterpret_cast<const f16x4*>(nv + 4 * j);
+      }
+    }
 
+    float m = kNegBig, l = 0.f;
+    f32x4 acc[kT];
+#pragma unroll
+    for (int i = 0; i < kT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    // id of page p of this window or the next one
+    auto page_id = [&](int p) { return __builtin_amdgcn_readlane((p >> 6) == win ? ids0 : ids1, p & 63); };
+    auto page_scale = [&](float x, int p) {  // (of this window)
+      return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), p & 63));
+    };
     auto issue_page = [&](int p, F8Page<D>& r) __attribute__((always_inline)) {
-      const int id = max(__builtin_amdgcn_readlane(ids, p - win), 0);
+      const int raw = page_id(p), id = in_pool(raw) ? raw : 0;
       const uint8_t* kb = cache.codes + f8_block<D>(id, hkv, h);
       const uint8_t* vb = kb + v_codes;
 #pragma unroll
@@ -246,34 +373,16 @@ __global__ __launch_bounds__(kF8DecThreads) void decode_fp8_kernel(
         }
       }
     };
-
-    float m = kNegBig, l = 0.f;
-    f32x4 acc[kT];
-#pragma unroll
-    for (int i = 0; i < kT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int last = np - 1;
 
     // The step's token into the row's last page, in registers: new scales, codes, and the stores.
-    auto append = [&](F8Page<D>& r, float& ks, float& vs, int id) {
+    auto append = [&](F8Page<D>& r, float& ks, float& vs, int id) __attribute__((always_inline)) {
       const int off = (len - 1) % kF8Page;
-      const f16* nk = ap.new_k + (int64_t(b) * hkv + h) * D;
-      const f16* nv = ap.new_v + (int64_t(b) * hkv + h) * D;
-      f16x8 xk[2 * kKL];
       float ka = 0.f, va = 0.f;
 #pragma unroll
-      for (int i = 0; i < kKL; ++i) {
-        xk[2 * i] = as_h8(ld16(nk + 64 * i + 16 * g));
-        xk[2 * i + 1] = as_h8(ld16(nk + 64 * i + 16 * g + 8));
-      }
-      f16 xv[4 * kVW];
+      for (int j = 0; j < kVW; ++j)
 #pragma unroll
-      for (int j = 0; j < 4 * kVW; j += 4) {
-        const f16x4 x = *reinterpret_cast<const f16x4*>(nv + n * (D / 16) + j);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          xv[j + c] = x[c];
-          va = fmaxf(va, fabsf(float(x[c])));
-        }
-      }
+        for (int c = 0; c < 4; ++c) va = fmaxf(va, fabsf(float(xv[j][c])));
 #pragma unroll
       for (int i = 0; i < 2 * kKL; ++i) ka = fmaxf(ka, f8_amax8(xk[i]));
       ka = max_lane32(swap_max16(ka));
@@ -302,8 +411,7 @@ __global__ __launch_bounds__(kF8DecThreads) void decode_fp8_kernel(
       }
 #pragma unroll
       for (int j = 0; j < kVW; ++j) {
-        const uint32_t c = f8_pack(float(xv[4 * j]) * vi, float(xv[4 * j + 1]) * vi, float(xv[4 * j + 2]) * vi,
-                                   float(xv[4 * j + 3]) * vi);
+        const uint32_t c = f8_pack(float(xv[j][0]) * vi, float(xv[j][1]) * vi, float(xv[j][2]) * vi, float(xv[j][3]) * vi);
 #pragma unroll
         for (int t = 0; t < 4; ++t)
           if (4 * g + t == off) r.v[t][j] = c;
@@ -330,231 +438,274 @@ __global__ __launch_bounds__(kF8DecThreads) void decode_fp8_kernel(
       vs = vs1;
     };
 
-    // Pages p and p + 1 (two: whether the second is in the piece).
-    auto consume = [&](int p, bool two, F8Page<D>& r0, F8Page<D>& r1) __attribute__((always_inline)) {
-      f32x4 s[2];
-      float vs[2];
-      bool live[2];
+    float ksc = 0.f, vsc = 0.f;
+    // Page p of the piece.  tail: its last page, which may end inside, and where the step's token may belong.
+    auto consume = [&](int p, F8Page<D>& r, auto tail_t) __attribute__((always_inline)) {
+      constexpr bool tail = decltype(tail_t)::value;
+      const int id = __builtin_amdgcn_readlane(ids0, p & 63);
+      const int left = !in_pool(id) ? 0 : tail ? len - (a + p) * kF8Page : kF8Page;  // tokens of the page that are attended
+      float ks = page_scale(ksc, p), vs = page_scale(vsc, p);
+      if constexpr (kAppend && tail) {
+        if (appends && in_pool(id)) append(r, ks, vs, id);
+      }
+      f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        F8Page<D>& r = x == 0 ? r0 : r1;
-        const int at = x == 0 || two ? p + x - win : p - win;
-        const int id = __builtin_amdgcn_readlane(ids, at);
-        live[x] = id >= 0 && (x == 0 || two);
-        float ks = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ksc), at));
-        vs[x] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vsc), at));
-        if constexpr (kAppend) {
-          if (live[x] && p + x == npages - 1 && row_len <= cap) append(r, ks, vs[x], id);
-        }
-        s[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int c = 0; c < kKL; ++c) {
 #pragma unroll
-        for (int i = 0; i < kKL; ++i) {
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint32_t w0 = r.k[i][2 * half], w1 = r.k[i][2 * half + 1];
-            const f16x2 h0 = f8_to_f16<false>(w0, ks), h1 = f8_to_f16<true>(w0, ks), h2 = f8_to_f16<false>(w1, ks),
-                        h3 = f8_to_f16<true>(w1, ks);
-            s[x] = mfma16(f16x8{h0[0], h0[1], h1[0], h1[1], h2[0], h2[1], h3[0], h3[1]}, qf[2 * i + half], s[x]);
-          }
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t w0 = r.k[c][2 * half], w1 = r.k[c][2 * half + 1];
+          const f16x2 h0 = f8_to_f16<false>(w0, ks), h1 = f8_to_f16<true>(w0, ks), h2 = f8_to_f16<false>(w1, ks),
+                      h3 = f8_to_f16<true>(w1, ks);
+          s = mfma16(f16x8{h0[0], h0[1], h1[0], h1[1], h2[0], h2[1], h3[0], h3[1]}, qf[2 * c + half], s);
         }
       }
       // scores in base 2; tokens past the row's end, and of pages outside the pool, have none
-      float sv[8];
-      float mx = -INFINITY;
+      float sv[4];
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int left = live[x] ? len - (p + x) * kF8Page : 0;
-        if (left < kF8Page) {  // (uniform)
+      for (int j = 0; j < 4; ++j) sv[j] = s[j] * scale_log2;
+      if (left < kF8Page) {  // (uniform)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const bool in = 4 * g + j < left;
-            sv[4 * x + j] = in ? s[x][j] * scale_log2 : -INFINITY;
+        for (int j = 0; j < 4; ++j) {
+          const bool in = 4 * g + j < left;
+          sv[j] = in ? sv[j] : -INFINITY;
 #pragma unroll
-            for (int c = 0; c < kVW; ++c) {  // (their codes may be anything, and 0 x NaN is NaN)
-              uint32_t& w = (x == 0 ? r0 : r1).v[j][c];
-              w = in ? w : 0u;
-            }
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) sv[4 * x + j] = s[x][j] * scale_log2;
+          for (int c = 0; c < kVW; ++c) r.v[j][c] = in ? r.v[j][c] : 0u;  // (their codes may be anything, and 0 x NaN is NaN)
         }
       }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) mx = fmaxf(mx, sv[j]);
-      mx = max_lane32(swap_max16(mx));
+      const float mx = max_lane32(swap_max16(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]))));
       if (__builtin_amdgcn_ballot_w64(mx > m) != 0) {
         const float mn = fmaxf(m, mx);
         const float al = exp2_fast(m - mn);
         m = mn;
         l *= al;
 #pragma unroll
-        for (int i = 0; i < kT; ++i)
+        for (int t = 0; t < kT; ++t)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[i][j] *= al;
+          for (int j = 0; j < 4; ++j) acc[t][j] *= al;
       }
-      float pr[8];
+      float pr[4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) pr[j] = exp2_fast(sv[j] - m);
-      const float l0 = (pr[0] + pr[1]) + (pr[2] + pr[3]), l1 = (pr[4] + pr[5]) + (pr[6] + pr[7]);
-      l += l0 + l1;
+      for (int j = 0; j < 4; ++j) pr[j] = exp2_fast(sv[j] - m);
+      const float l0 = (pr[0] + pr[1]) + (pr[2] + pr[3]);
+      l += l0;
       if constexpr (kWeights) {
-        const float w0 = swap_sum(l0), w1 = swap_sum(l1);
-        if (g == 0 && n < G) {
-          float* dst = ws.lse + ((int64_t(b) * hkv + h) * max_pages + p) * G + n;
-          st_dev(dst, __builtin_amdgcn_logf(w0) + m);
-          if (two) st_dev(dst + G, __builtin_amdgcn_logf(w1) + m);
-        }
+        const float lw = __builtin_amdgcn_logf(swap_sum(l0)) + m;
+        if (g == 0 && n < G) my_lse[(p & 63) * G + n] = lw;
       }
-      const f16x8 pf = f16x8{f16(pr[0]), f16(pr[1]), f16(pr[2]), f16(pr[3]), f16(pr[4]), f16(pr[5]), f16(pr[6]), f16(pr[7])};
+      const f16x4 pf = f16x4{f16(pr[0]), f16(pr[1]), f16(pr[2]), f16(pr[3])};
 #pragma unroll
       for (int c = 0; c < kVW; ++c) {
-        uint32_t tr[2][4];  // byte transposes: word i = dim 4 c + i of tokens 4 g .. 4 g + 3
+        // byte transpose: word j = dim 4 c + j of tokens 4 g .. 4 g + 3
+        const uint32_t ab = __builtin_amdgcn_perm(r.v[1][c], r.v[0][c], 0x05010400u);
+        const uint32_t ab2 = __builtin_amdgcn_perm(r.v[1][c], r.v[0][c], 0x07030602u);
+        const uint32_t cd = __builtin_amdgcn_perm(r.v[3][c], r.v[2][c], 0x05010400u);
+        const uint32_t cd2 = __builtin_amdgcn_perm(r.v[3][c], r.v[2][c], 0x07030602u);
+        const uint32_t tr[4] = {__builtin_amdgcn_perm(cd, ab, 0x05040100u), __builtin_amdgcn_perm(cd, ab, 0x07060302u),
+                                __builtin_amdgcn_perm(cd2, ab2, 0x05040100u), __builtin_amdgcn_perm(cd2, ab2, 0x07060302u)};
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const F8Page<D>& r = x == 0 ? r0 : r1;
-          const uint32_t ab = __builtin_amdgcn_perm(r.v[1][c], r.v[0][c], 0x05010400u);
-          const uint32_t ab2 = __builtin_amdgcn_perm(r.v[1][c], r.v[0][c], 0x07030602u);
-          const uint32_t cd = __builtin_amdgcn_perm(r.v[3][c], r.v[2][c], 0x05010400u);
-          const uint32_t cd2 = __builtin_amdgcn_perm(r.v[3][c], r.v[2][c], 0x07030602u);
-          tr[x][0] = __builtin_amdgcn_perm(cd, ab, 0x05040100u);
-          tr[x][1] = __builtin_amdgcn_perm(cd, ab, 0x07060302u);
-          tr[x][2] = __builtin_amdgcn_perm(cd2, ab2, 0x05040100u);
-          tr[x][3] = __builtin_amdgcn_perm(cd2, ab2, 0x07060302u);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f16x2 h0 = f8_to_f16<false>(tr[0][i], vs[0]), h1 = f8_to_f16<true>(tr[0][i], vs[0]),
-                      h2 = f8_to_f16<false>(tr[1][i], vs[1]), h3 = f8_to_f16<true>(tr[1][i], vs[1]);
-          acc[4 * c + i] = mfma16(f16x8{h0[0], h0[1], h1[0], h1[1], h2[0], h2[1], h3[0], h3[1]}, pf, acc[4 * c + i]);
+        for (int j = 0; j < 4; ++j) {
+          const f16x2 h0 = f8_to_f16<false>(tr[j], vs), h1 = f8_to_f16<true>(tr[j], vs);
+          acc[4 * c + j] = mfma16(f16x4{h0[0], h0[1], h1[0], h1[1]}, pf, acc[4 * c + j]);
         }
       }
     };
+    // The page sums of a window go out together: whole lines, where a page's own are 4 G bytes (128 rows of 1023-8190
+    // keys, 32 / 8 heads: 249 us with a store for every four pages, 223 so, 213 without weights).
+    auto flush_lse = [&](int p0, int count) __attribute__((always_inline)) {
+      float* dst = ws.lse + ((int64_t(b) * hkv + h) * max_pages + a + p0) * G;
+      for (int x = lane; x < count * G; x += kWave) st_dev(dst + x, my_lse[x]);
+    };
 
-    F8Page<D> a0, a1, b0, b1;
-    for (int w0 = a; w0 < e; w0 += kWave) {  // windows of 64 pages
-      const int we = min(w0 + kWave, e);
-      if (w0 != a) load_window(w0);
-      const int steps = (we - w0 + 1) / 2;
-      auto issue = [&](int i, F8Page<D>& r0, F8Page<D>& r1) __attribute__((always_inline)) {
-        const int p = w0 + 2 * i;
-        issue_page(p, r0);
-        issue_page(min(p + 1, we - 1), r1);
-      };
-      auto step = [&](int i, F8Page<D>& r0, F8Page<D>& r1) __attribute__((always_inline)) {
-        consume(w0 + 2 * i, w0 + 2 * i + 1 < we, r0, r1);
-      };
-      issue(0, a0, a1);
-      int i = 0;
-      for (; i + 2 < steps; i += 2) {
-        issue(i + 1, b0, b1);
-        __builtin_amdgcn_sched_barrier(0);
-        step(i, a0, a1);
-        issue(i + 2, a0, a1);
-        __builtin_amdgcn_sched_barrier(0);
-        step(i + 1, b0, b1);
+    // Ring of S pages: page p + S - 1 is requested while page p is attended.  Past the piece's end the last page is
+    // requested again, so that the loads in flight are a fixed number and no wait is for more than one page.
+    F8Page<D> r[S], rt;
+    const std::integral_constant<bool, false> mid{};
+    const std::integral_constant<bool, true> end{};
+    settle(ids0, ids1);
+    ksc = load_scale(ids0, 0);
+    vsc = load_scale(ids0, v_scales);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int x = 0; x < S - 1; ++x) issue_page(min(x, last), r[x]);
+    __builtin_amdgcn_sched_barrier(0);
+    settle(ksc, vsc);
+    int p = 0;
+    for (;; ++win) {  // one window of pages; the next one's scales and the one after's ids are on their way meanwhile
+      float k_next = 0.f, v_next = 0.f;
+      int id_next = 0;
+      const bool more = (win + 1) * kWave <= last;
+      if (more) {
+        k_next = load_scale(ids1, 0);
+        v_next = load_scale(ids1, v_scales);
+        id_next = load_ids(win + 2);
       }
-      if (i + 1 < steps) {
-        issue(i + 1, b0, b1);
+      const int stop = min(last, (win + 1) * kWave);
+      for (; p + S <= stop; p += S) {
+#pragma unroll
+        for (int x = 0; x < S; ++x) {
+          issue_page(min(p + x + S - 1, last), r[(x + S - 1) % S]);
+          __builtin_amdgcn_sched_barrier(0);
+          consume(p + x, r[x], mid);
+        }
+      }
+      if (!more) break;
+      if constexpr (kWeights) flush_lse(win * kWave, kWave);
+      ids0 = ids1;
+      ids1 = id_next;
+      ksc = k_next;
+      vsc = v_next;
+      settle(ids0, ids1);
+      settle(ksc, vsc);
+    }
+#pragma unroll
+    for (int x = 0; x < S; ++x) {
+      if (p + x < last) {
+        if (p + x + S - 1 <= last) issue_page(p + x + S - 1, r[(x + S - 1) % S]);
         __builtin_amdgcn_sched_barrier(0);
-        step(i, a0, a1);
-        step(i + 1, b0, b1);
-      } else {
-        step(i, a0, a1);
+        consume(p + x, r[x], mid);
+      } else if (p + x == last) {
+        rt = r[x];
       }
     }
+    consume(last, rt, end);
+    if constexpr (kWeights) flush_lse(win * kWave, np - win * kWave);
 
+    const int first = range_of(cb), nranges = range_of(cb + npages - 1) - first + 1;
     l = swap_sum(l);
     if (nranges == 1) {
       const float inv = l > 0.f ? 1.f / l : 0.f;
       if (n < G) {
         f16* op = out + (int64_t(b) * hq + h * G + n) * D + 4 * g * (D / 16);
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+        for (int x = 0; x < 4; ++x)
 #pragma unroll
           for (int c = 0; c < kVW; ++c)
-            *reinterpret_cast<f16x4*>(op + r * (D / 16) + 4 * c) =
-                f16x4{f16(acc[4 * c][r] * inv), f16(acc[4 * c + 1][r] * inv), f16(acc[4 * c + 2][r] * inv),
-                      f16(acc[4 * c + 3][r] * inv)};
+            *reinterpret_cast<f16x4*>(op + x * (D / 16) + 4 * c) =
+                f16x4{f16(acc[4 * c][x] * inv), f16(acc[4 * c + 1][x] * inv), f16(acc[4 * c + 2][x] * inv),
+                      f16(acc[4 * c + 3][x] * inv)};
       }
       if constexpr (kWeights) {
         wait_all_mem();  // (this wave's own lse stores)
-        add_weights(b, l > 0.f ? m + __builtin_amdgcn_logf(l) : INFINITY, npages);
+        const float tot = l > 0.f ? m + __builtin_amdgcn_logf(l) : INFINITY;
+        add_weights(b, [&](int x) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, tot), x)); },
+                    npages, lane, kWave);
       }
     } else {
-      const int64_t slot = (int64_t(b) + stream) * hkv + h;
+      const int en = 2 * wv + npend;
       if (n < G) {
-        if (g == 0) st_dev8(ws.ml + (slot * G + n) * 2, f32x2{m, l});
-        float* so = ws.o + slot * G * D;
+        if (g == 0) {
+          s_m[en][n] = m;
+          s_l[en][n] = l;
+        }
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+        for (int x = 0; x < 4; ++x)
 #pragma unroll
-          for (int c = 0; c < kVW; ++c) {
-            float* dst = so + ((r * kVW + c) * 4 * G + g * G + n) * 4;
-            st_dev8(dst, f32x2{acc[4 * c][r], acc[4 * c + 1][r]});
-            st_dev8(dst + 2, f32x2{acc[4 * c + 2][r], acc[4 * c + 3][r]});
-          }
+          for (int c = 0; c < kVW; ++c)
+            s_o[en * units + (x * kVW + c) * 4 * G + g * G + n] = f32x4{acc[4 * c][x], acc[4 * c + 1][x], acc[4 * c + 2][x], acc[4 * c + 3][x]};
       }
-      pend_b[npend & 1] = b;  // (only the first and the last piece of a range can be split)
-      pend_f[npend & 1] = first;
-      pend_np[npend & 1] = nranges;
+      if (lane == 0) {
+        s_row[en] = b;
+        s_first[en] = first;
+        s_last[en] = first + nranges - 1;
+      }
       ++npend;
     }
   }
 
-  for (int x = 0; x < npend; ++x) {
-    const int b = x == 0 ? pend_b[0] : pend_b[1], np = x == 0 ? pend_np[0] : pend_np[1];
-    const int first = x == 0 ? pend_f[0] : pend_f[1];
-    uint32_t* ticket = ws.count + int64_t(b) * hkv + h;
-    if (!wave_arrive_last(ticket, uint32_t(np - 1), lane)) continue;
-    const int64_t slot0 = (int64_t(b) + first) * hkv + h;  // state j: slot0 + j hkv
-    // totals of query n % G
-    float M = kNegBig, L = 0.f;
-    const int nn = min(n, G - 1);
-    for (int j = 0; j < np; ++j) {
-      const f32x2 ml = ld_dev8(ws.ml + ((slot0 + int64_t(j) * hkv) * G + nn) * 2);
-      const float mn = fmaxf(M, ml[0]);
-      L = L * exp2_fast(M - mn) + ml[1] * exp2_fast(ml[0] - mn);
-      M = mn;
+  // The workgroup's states, in range order: those of one row are merged; a row that only this workgroup holds is
+  // done, the others' states (the first and the last row's, at most) are published.
+  if constexpr (kWeights) wait_all_mem();
+  __syncthreads();
+  const int tid = threadIdx.x;
+  auto write_unit = [&](int b, int u, f32x4 o, float inv) {
+    const int cl = u % (4 * G), un = cl % G, ug = cl / G, i4 = u / (4 * G);
+    *reinterpret_cast<f16x4*>(out + (int64_t(b) * hq + h * G + un) * D + (4 * ug + i4 / kVW) * (D / 16) + 4 * (i4 % kVW)) =
+        f16x4{f16(o[0] * inv), f16(o[1] * inv), f16(o[2] * inv), f16(o[3] * inv)};
+  };
+  auto row_weights = [&](int b) {  // s_tot holds the row's totals
+    __syncthreads();
+    add_weights(b, [&](int x) { return s_tot[x]; }, s_cum[b + 1] - s_cum[b] - kRowStart, tid, kWaves * kWave);
+    __syncthreads();
+  };
+  int open = 0, open_b[2] = {0, 0}, open_wg[2] = {0, 0}, open_np[2] = {0, 0};
+  for (int e0 = 0; e0 < kEnt;) {
+    const int b = s_row[e0];
+    if (b < 0) {
+      ++e0;
+      continue;
     }
-    const float inv = L > 0.f ? 1.f / L : 0.f;
-    for (int u0 = 0; u0 < kU * 4 * G; u0 += kWave) {  // 4-dim units: (r kVW + c) 4 G + g G + n
-      const int u = u0 + lane;
-      const bool on = u < kU * 4 * G;
-      const int cl = u % (4 * G), un = cl % G, ug = cl / G, i4 = u / (4 * G);
-      const float Mu = __shfl(M, un), iu = __shfl(inv, un);
+    int e1 = e0 + 1;
+    while (e1 < kEnt && (s_row[e1] == b || s_row[e1] < 0)) ++e1;
+    const int wg0 = s_first[e0] / kWaves, wg1 = s_last[e0] / kWaves;
+    const bool whole = wg0 == wg1;
+    for (int u = tid; u < units; u += kWaves * kWave) {
+      const int un = u % (4 * G) % G;
+      float M = kNegBig, L = 0.f;
       f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (on) {
-        for (int j = 0; j < np; ++j) {
-          const int64_t sl = slot0 + int64_t(j) * hkv;
-          const float w = exp2_fast(ld_dev(ws.ml + (sl * G + un) * 2) - Mu);
-          const float* src = ws.o + sl * G * D + u * 4;
-          const f32x2 x0 = ld_dev8(src), x1 = ld_dev8(src + 2);
-          o = f32x4{fmaf(w, x0[0], o[0]), fmaf(w, x0[1], o[1]), fmaf(w, x1[0], o[2]), fmaf(w, x1[1], o[3])};
-        }
-        *reinterpret_cast<f16x4*>(out + (int64_t(b) * hq + h * G + un) * D + (4 * ug + i4 / kVW) * (D / 16) + 4 * (i4 % kVW)) =
-            f16x4{f16(o[0] * iu), f16(o[1] * iu), f16(o[2] * iu), f16(o[3] * iu)};
+      for (int x = e0; x < e1; ++x)
+        if (s_row[x] == b) M = fmaxf(M, s_m[x][un]);
+      for (int x = e0; x < e1; ++x) {
+        if (s_row[x] != b) continue;
+        const float w = exp2_fast(s_m[x][un] - M);
+        const f32x4 v = s_o[x * units + u];
+        L = fmaf(w, s_l[x][un], L);
+        o = f32x4{fmaf(w, v[0], o[0]), fmaf(w, v[1], o[1]), fmaf(w, v[2], o[2]), fmaf(w, v[3], o[3])};
+      }
+      if (whole) {
+        write_unit(b, u, o, L > 0.f ? 1.f / L : 0.f);
+        if (kWeights && u < G) s_tot[u] = L > 0.f ? M + __builtin_amdgcn_logf(L) : INFINITY;
+      } else {
+        const uint32_t slot = uint32_t((int64_t(b) + wg) * hkv + h);
+        st_dev4(r_o, (slot * G * D + u * 4) * 4, o);
+        if (u < G) st_dev2(r_ml, (slot * G + u) * 8, f32x2{M, L});
       }
     }
-    if constexpr (kWeights) {
-      const int npages = s_cum[b + 1] - s_cum[b] - kRowStart;
-      add_weights(b, L > 0.f ? M + __builtin_amdgcn_logf(L) : INFINITY, __builtin_amdgcn_readfirstlane(npages));
+    if (whole) {
+      if constexpr (kWeights) row_weights(b);
+    } else {
+      open_b[open & 1] = b;
+      open_wg[open & 1] = wg0;
+      open_np[open & 1] = wg1 - wg0 + 1;
+      ++open;
     }
-    if (lane == 0) reset_ticket(ticket);
+    e0 = e1;
+  }
+  if (open == 0) return;
+  wait_all_mem();
+  __syncthreads();
+  if (tid < open)
+    s_ticket[tid] = __hip_atomic_fetch_add(ws.count + int64_t(tid == 0 ? open_b[0] : open_b[1]) * hkv + h, 1u,
+                                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  compiler_fence();  // the merge loads below stay behind the tickets
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    if (x >= open || s_ticket[x] != uint32_t(open_np[x] - 1)) continue;
+    const int b = open_b[x];
+    const int64_t slot0 = (int64_t(b) + open_wg[x]) * hkv + h;  // state j: slot0 + j hkv
+    for (int u = tid; u < units; u += kWaves * kWave) {
+      float M, L;
+      f32x4 o;
+      f8_merge(r_ml, r_o, slot0, hkv, open_np[x], G, D, u % (4 * G) % G, u, M, L, o);
+      write_unit(b, u, o, L > 0.f ? 1.f / L : 0.f);
+      if (kWeights && u < G) s_tot[u] = L > 0.f ? M + __builtin_amdgcn_logf(L) : INFINITY;
+    }
+    if constexpr (kWeights) row_weights(b);
+    if (tid == 0) reset_ticket(ws.count + int64_t(b) * hkv + h);
   }
 }
 
-// Streams of a call: at most one wave per kv head and stream, kF8WavesPerCu waves a CU, and no more than the
-// longest call of these sizes has ranges.
-constexpr int kF8WavesPerCu = 8;
+// Streams of a call, whole workgroups of them: at most kWavesPerCu waves a CU over all kv heads, and no more than
+// the longest call of these sizes has ranges.
+constexpr int kWavesPerCu = 8;
 static int64_t f8_streams(int64_t batch, int32_t hkv, int32_t max_len, int cus) {
-  const int64_t most = ceil_div(batch * (ceil_div(max_len, kF8Page) + kRowStart), kMinPages);
-  const int64_t waves = int64_t(cus) * kF8WavesPerCu;
-  return std::max<int64_t>(1, std::min(most, std::max<int64_t>(1, waves / hkv)));
+  const int64_t most = ceil_div(ceil_div(batch * (ceil_div(max_len, kF8Page) + kRowStart), kMinPages), kDecWaves);
+  const int64_t wgs = int64_t(cus) * kWavesPerCu / kDecWaves / hkv;
+  return kDecWaves * std::max<int64_t>(1, std::min(most, wgs));
 }
-static size_t f8_ws_layout(int64_t batch, int64_t streams, int32_t hkv, int32_t G, int32_t d, int32_t max_pages,
+static size_t f8_ws_layout(int64_t batch, int64_t wgs, int32_t hkv, int32_t G, int32_t d, int32_t max_pages,
                            bool weights, size_t* off_ml, size_t* off_o, size_t* off_lse) {
-  const size_t slots = size_t(batch + streams) * hkv * G;
+  const size_t slots = size_t(batch + wgs) * hkv * G;
   size_t off = kTicketBytes;
   *off_ml = off;
   off = align256(off + slots * 2 * sizeof(float));
@@ -595,7 +746,7 @@ static int f8_decode(void* out, const void* query, void* codes, float* scales, i
   IFN_CHECK_ALIGN16(workspace);
   const int64_t streams = f8_streams(batch, hkv, cap, std::max(1, cus));
   size_t off_ml, off_o, off_lse;
-  if (workspace_bytes < f8_ws_layout(batch, streams, hkv, G, d, max_pages, page_weights != nullptr, &off_ml, &off_o,
+  if (workspace_bytes < f8_ws_layout(batch, streams / kDecWaves, hkv, G, d, max_pages, page_weights != nullptr, &off_ml, &off_o,
                                      &off_lse))
     return IFN_ERR_WORKSPACE;
   if (cus < 1) return IFN_ERR_HIP;
@@ -605,10 +756,12 @@ static int f8_decode(void* out, const void* query, void* codes, float* scales, i
   const F8Cache cache{static_cast<uint8_t*>(codes), scales, num_pages};
   const F8Append ap{static_cast<const f16*>(new_k), static_cast<const f16*>(new_v)};
   const float sl = (scale > 0.f ? scale : 1.f / sqrtf(float(d))) * kLog2e;
-  const int64_t blocks = ceil_div(streams * hkv, kF8DecWaves);
+  const int64_t blocks = streams / kDecWaves * hkv;
+  const size_t lds = size_t(2 * kDecWaves) * G * d * sizeof(float) + size_t(batch + 1) * sizeof(int) +
+                     (page_weights != nullptr ? size_t(kDecWaves) * kWave * G * sizeof(float) : 0);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   auto launch = [&](auto k) {
-    k<<<dim3(unsigned(blocks)), dim3(kF8DecThreads), 0, s>>>(
+    k<<<dim3(unsigned(blocks)), dim3(kDecThreads), lds, s>>>(
         static_cast<f16*>(out), static_cast<const f16*>(query), cache, block_tables, max_pages, seq_lens, active, batch,
         hkv, G, cap, sl, ws, ap, page_weights, int32_t(streams));
   };
@@ -635,9 +788,9 @@ extern "C" size_t ifn_paged_decode_fp8_workspace_bytes(int32_t batch, int32_t nu
       block_size < 1 || max_pages_per_seq < 1 || max_seq_len < 0)
     return 0;
   const int64_t cap = std::min<int64_t>(int64_t(max_pages_per_seq) * kF8Page, max_seq_len);
-  const int64_t streams = f8_streams(batch, num_kv_heads, int32_t(cap), std::max(1, device_cu_count()));
+  const int64_t wgs = f8_streams(batch, num_kv_heads, int32_t(cap), std::max(1, device_cu_count())) / kDecWaves;
   size_t a, b, c;
-  return f8_ws_layout(batch, streams, num_kv_heads, num_q_heads / num_kv_heads, head_dim, max_pages_per_seq,
+  return f8_ws_layout(batch, wgs, num_kv_heads, num_q_heads / num_kv_heads, head_dim, max_pages_per_seq,
                       page_weights != 0, &a, &b, &c);
 }
 

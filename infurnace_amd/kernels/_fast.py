@@ -15,7 +15,8 @@ import warnings
 from .. import _capi
 
 EXT_PATH = os.path.join(os.path.dirname(_capi.LIB_PATH), "_fast_call.so")
-_NAMES = ("decode", "prep_decode", "prefill", "prep_prefill", "prep_append", "store", "store_layers")
+_NAMES = ("decode", "prep_decode", "prefill", "prep_prefill", "prep_append", "store", "store_layers", "store_fp8",
+          "decode_fp8", "prefill_fp8", "evict")
 # the C entry points the extension calls, in the order it takes their addresses
 _ENTRIES = ("ifn_store_kv", "ifn_store_kv_layers", "ifn_paged_decode_workspace_bytes",
             "ifn_paged_decode_plan_bytes", "ifn_paged_decode",
@@ -24,7 +25,8 @@ _ENTRIES = ("ifn_store_kv", "ifn_store_kv_layers", "ifn_paged_decode_workspace_b
             "ifn_paged_decode_shared_prefix_workspace_bytes", "ifn_paged_decode_shared_prefix",
             "ifn_paged_prefill_workspace_bytes", "ifn_paged_prefill", "ifn_paged_prefill_append",
             "ifn_qk_norm_rope_append", "ifn_paged_decode_prep_append", "ifn_paged_decode_prep_append_planning",
-            "ifn_paged_prefill_prep_append")
+            "ifn_paged_prefill_prep_append", "ifn_store_kv_fp8", "ifn_paged_decode_fp8_workspace_bytes",
+            "ifn_paged_decode_fp8", "ifn_paged_decode_append_fp8", "ifn_paged_prefill_fp8", "ifn_evict_pages")
 
 
 def _none(*args):
@@ -66,4 +68,5 @@ def _first(name):
     return call
 
 
-decode, prep_decode, prefill, prep_prefill, prep_append, store, store_layers = (_first(n) for n in _NAMES)
+(decode, prep_decode, prefill, prep_prefill, prep_append, store, store_layers, store_fp8, decode_fp8, prefill_fp8,
+ evict) = (_first(n) for n in _NAMES)

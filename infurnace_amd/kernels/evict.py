@@ -9,6 +9,7 @@ from __future__ import annotations
 import torch
 
 from .. import _capi
+from . import _fast
 from ._carrier import accepts_carriers
 from ._common import PagedAttentionError, current_stream, ptr
 from .kv_fp8 import _current
@@ -17,7 +18,6 @@ from .paged_attention import _check
 __all__ = ["evict_pages"]
 
 
-@accepts_carriers
 def evict_pages(block_tables: torch.Tensor, sequence_lengths: torch.Tensor, page_weights: torch.Tensor, keep_pages: int,
                 *, sink_pages: int = 1, recent_pages: int = 1, active_mask: torch.Tensor | None = None,
                 block_size: int = 16) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -31,6 +31,16 @@ def evict_pages(block_tables: torch.Tensor, sequence_lengths: torch.Tensor, page
     (``num_evicted`` int32 [B] of them), for the caller to release.  Tokens keep the rotary positions they were
     stored with; the length only counts what is held.  No page is moved or written, so shared pages are safe.
     """
+    got = _fast.evict(block_tables, sequence_lengths, page_weights, keep_pages, sink_pages, recent_pages, active_mask,
+                      block_size)
+    if got is not None:
+        return got
+    return _evict(block_tables, sequence_lengths, page_weights, keep_pages, sink_pages, recent_pages, active_mask,
+                  block_size)
+
+
+@accepts_carriers
+def _evict(block_tables, sequence_lengths, page_weights, keep_pages, sink_pages, recent_pages, active_mask, block_size):
     err = PagedAttentionError
     if not isinstance(block_tables, torch.Tensor) or block_tables.ndim != 2:
         raise err("block_tables must be a rank-2 [B, max_pages] int32 tensor")

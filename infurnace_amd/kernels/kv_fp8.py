@@ -24,9 +24,10 @@ import math
 import torch
 
 from .. import _capi
+from . import _fast
 from ._carrier import accepts_carriers
 from ._common import KVStoreError, PagedAttentionError, current_stream, ptr
-from .paged_attention import _check, _row_keys, _validate_pages, workspace_for
+from .paged_attention import _WORKSPACES, _check, _row_keys, _validate_pages, workspace_for
 
 __all__ = ["store_kv_fp8", "paged_attention_fp8", "store_kv_fp8_and_decode", "EMPTY_SCALE"]
 
@@ -123,7 +124,6 @@ def _validate_scales(scales: torch.Tensor, table: torch.Tensor, keys: torch.Tens
         raise PagedAttentionError("scales of pages that are read must be positive powers of two")
 
 
-@accepts_carriers
 def store_kv_fp8(kv_pool: torch.Tensor, scales: torch.Tensor, slot_mapping: torch.Tensor,
                  active_mask: torch.Tensor | None, new_k: torch.Tensor, new_v: torch.Tensor, *, layer: int = 0,
                  validate: bool = False) -> None:
@@ -135,6 +135,13 @@ def store_kv_fp8(kv_pool: torch.Tensor, scales: torch.Tensor, slot_mapping: torc
     (every chunk and every step does); of two rows with one slot the later is stored.  ``validate=True``
     adds a synchronising host check of the slots.
     """
+    if not validate and _fast.store_fp8(kv_pool, scales, slot_mapping, active_mask, new_k, new_v, layer) is not None:
+        return None
+    return _store(kv_pool, scales, slot_mapping, active_mask, new_k, new_v, layer, validate)
+
+
+@accepts_carriers
+def _store(kv_pool, scales, slot_mapping, active_mask, new_k, new_v, layer, validate) -> None:
     pool_layer, scales_layer, (P, hkv, d) = _check_cache(kv_pool, scales, layer, KVStoreError)
     dev = pool_layer.device
     if not isinstance(new_k, torch.Tensor) or new_k.ndim != 3:
@@ -156,6 +163,7 @@ def store_kv_fp8(kv_pool: torch.Tensor, scales: torch.Tensor, slot_mapping: torc
                    T, hkv, d, BLOCK, current_stream(dev))
 
 
+@accepts_carriers
 def _decode(query, kv_pool, scales, block_tables, sequence_lengths, active_mask, new_k, new_v, append, layer, scale, out,
             max_seq_len, page_weights, validate):
     err = PagedAttentionError
@@ -214,7 +222,6 @@ def _decode(query, kv_pool, scales, block_tables, sequence_lengths, active_mask,
     return out
 
 
-@accepts_carriers
 def paged_attention_fp8(query: torch.Tensor, kv_pool: torch.Tensor, scales: torch.Tensor, block_tables: torch.Tensor,
                         sequence_lengths: torch.Tensor | None, active_mask: torch.Tensor | None = None, *,
                         layer: int = 0, scale: float | None = None, query_start: int | None = None,
@@ -236,8 +243,25 @@ def paged_attention_fp8(query: torch.Tensor, kv_pool: torch.Tensor, scales: torc
     are powers of two.
     """
     if query_start is None:
+        if not validate:
+            o = _fast.decode_fp8(query, kv_pool, scales, block_tables, sequence_lengths, active_mask, None, None, layer,
+                                 scale, out, max_seq_len, page_weights, _WORKSPACES)
+            if o is not None:
+                return o
         return _decode(query, kv_pool, scales, block_tables, sequence_lengths, active_mask, None, None, False, layer,
                        scale, out, max_seq_len, page_weights, validate)
+    if (sequence_lengths is None and active_mask is None and max_seq_len is None and page_weights is None and
+            not validate):
+        o = _fast.prefill_fp8(query, kv_pool, scales, block_tables, query_start, layer, scale, out)
+        if o is not None:
+            return o
+    return _prefill(query, kv_pool, scales, block_tables, sequence_lengths, active_mask, layer, scale, query_start, out,
+                    max_seq_len, page_weights, validate)
+
+
+@accepts_carriers
+def _prefill(query, kv_pool, scales, block_tables, sequence_lengths, active_mask, layer, scale, query_start, out,
+             max_seq_len, page_weights, validate):
     err = PagedAttentionError
     pool_layer, scales_layer, (P, hkv, d) = _check_cache(kv_pool, scales, layer, err)
     dev = pool_layer.device
@@ -281,7 +305,6 @@ def paged_attention_fp8(query: torch.Tensor, kv_pool: torch.Tensor, scales: torc
     return out
 
 
-@accepts_carriers
 def store_kv_fp8_and_decode(query: torch.Tensor, kv_pool: torch.Tensor, scales: torch.Tensor, block_tables: torch.Tensor,
                             sequence_lengths: torch.Tensor, active_mask: torch.Tensor | None, new_k: torch.Tensor,
                             new_v: torch.Tensor, *, layer: int = 0, scale: float | None = None,
@@ -294,5 +317,10 @@ def store_kv_fp8_and_decode(query: torch.Tensor, kv_pool: torch.Tensor, scales: 
     are inactive, empty or longer than ``max_seq_len`` store nothing.  A row's last page must be in no other
     row's table (true of any paged KV state).
     """
+    if not validate and new_k is not None:
+        o = _fast.decode_fp8(query, kv_pool, scales, block_tables, sequence_lengths, active_mask, new_k, new_v, layer,
+                             scale, out, max_seq_len, page_weights, _WORKSPACES)
+        if o is not None:
+            return o
     return _decode(query, kv_pool, scales, block_tables, sequence_lengths, active_mask, new_k, new_v, True, layer, scale,
                    out, max_seq_len, page_weights, validate)
