@@ -574,16 +574,22 @@ int ifn_paged_decode_append_fp8(void* out, const void* query, void* codes_layer,
                                 int32_t max_seq_len, float scale, void* workspace, size_t workspace_bytes,
                                 void* stream);
 
+/* Workspace bytes of the call below. */
+size_t ifn_paged_prefill_fp8_workspace_bytes(int32_t num_q_tokens, int32_t query_start,
+                                             int32_t num_q_heads, int32_t num_kv_heads,
+                                             int32_t head_dim, int32_t block_size);
+
 /*
  * ifn_paged_prefill over the 8-bit cache (the chunk's K/V stored before it).
- * Any group size; no workspace.
+ * Any group size.  The workspace follows the same zero-once rule as
+ * ifn_paged_decode.
  * Replaces: paged_attention with a multi-token query, docs/architecture.md:246.
  */
 int ifn_paged_prefill_fp8(void* out, const void* query, const void* codes_layer, const float* scales_layer,
                           int64_t num_pages, const int32_t* block_table, int32_t max_pages,
                           int32_t query_start, int32_t num_q_tokens, int32_t num_q_heads,
                           int32_t num_kv_heads, int32_t head_dim, int32_t block_size, float scale,
-                          void* stream);
+                          void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Eviction by accumulated attention weight: row b of n = ceil(seq_lens[b] / 16)

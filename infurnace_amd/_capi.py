@@ -92,9 +92,11 @@ SIGNATURES: dict[str, tuple] = {
                                             _i32, _f32, _p, _sz, _p]),
     "ifn_paged_decode_append_fp8": (ctypes.c_int, [_p, _p, _p, _p, _i64, _p, _i32, _p, _p, _p, _p, _p, _i32, _i32,
                                                    _i32, _i32, _i32, _i32, _f32, _p, _sz, _p]),
-    # out, q, codes, scales, num_pages, table, max_pages, query_start, T, hq, hkv, head_dim, block_size, scale, stream
+    "ifn_paged_prefill_fp8_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32]),
+    # out, q, codes, scales, num_pages, table, max_pages, query_start, T, hq, hkv, head_dim, block_size, scale,
+    # workspace, bytes, stream
     "ifn_paged_prefill_fp8": (ctypes.c_int, [_p, _p, _p, _p, _i64, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32,
-                                             _p]),
+                                             _p, _sz, _p]),
     # out_tables, out_lens, out_weights, num_evicted, tables, max_pages, lens, active, weights, batch, hkv, block_size,
     # keep, sink, recent, stream
     "ifn_evict_pages": (ctypes.c_int, [_p, _p, _p, _p, _p, _i32, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _p]),

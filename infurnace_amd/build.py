@@ -49,6 +49,7 @@ DEVICE_FLAGS = [
 FILE_FLAGS = {
     "paged_prefill_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-fno-honor-nans"],
     "paged_prefill_block.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-fno-honor-nans"],
+    "paged_prefill_fp8_block.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-fno-honor-nans"],
     # The whole-row decode kernel's first nine arguments (plan, pool, tables, query, sizes, grid) are
     # preloaded into scalar registers at dispatch, so its first loads (the step plan) do not wait
     # for the kernel-argument loads.

@@ -41,7 +41,8 @@ namespace {
   X(prep_decode, ifn_paged_decode_prep_append) X(prep_decode_planning, ifn_paged_decode_prep_append_planning) \
   X(prep_prefill, ifn_paged_prefill_prep_append) X(store_fp8, ifn_store_kv_fp8) \
   X(decode_fp8_ws, ifn_paged_decode_fp8_workspace_bytes) X(decode_fp8, ifn_paged_decode_fp8) \
-  X(decode_append_fp8, ifn_paged_decode_append_fp8) X(prefill_fp8, ifn_paged_prefill_fp8) \
+  X(decode_append_fp8, ifn_paged_decode_append_fp8) \
+  X(prefill_fp8_ws, ifn_paged_prefill_fp8_workspace_bytes) X(prefill_fp8, ifn_paged_prefill_fp8) \
   X(evict_pages, ifn_evict_pages)
 struct Entries {
 #define IFN_MEMBER(name, fn) decltype(&fn) name;
@@ -596,7 +597,7 @@ PyObject* decode_fp8(PyObject* const* a) {
   return done(out, a[10]);
 }
 
-// prefill_fp8(query, kv_pool, scales, block_table, query_start, layer, scale, out)
+// prefill_fp8(query, kv_pool, scales, block_table, query_start, layer, scale, out, workspaces)
 PyObject* prefill_fp8(PyObject* const* a) {
   const Cache P = cache8(a[1], a[2], integer(a[5]));
   const at::Tensor& q = tensor(a[0], at::kHalf, P.dev);
@@ -606,10 +607,13 @@ PyObject* prefill_fp8(PyObject* const* a) {
   const at::Tensor& bt = table_of(a[3], P.dev, mp);
   need(start >= 0 && start + n <= mp * P.bs);
   const float scale = scale_of(a[6], P.d);
+  const int32_t N = small(n), Q = small(hq);
+  const Call w = call_on(a[8], P.dev, E.prefill_fp8_ws(N, int32_t(start), Q, P.hkv, P.d, P.bs));
+  need(!capturing(w.stream));
   const at::Tensor out = output(a[7], P, n, hq, false);
   launched(launch(E.prefill_fp8, out.data_ptr(), q.data_ptr(), P.p, P.scales, P.pages,
-                  static_cast<const int32_t*>(bt.data_ptr()), small(mp), int32_t(start), small(n), small(hq), P.hkv, P.d,
-                  P.bs, scale, stream_of(P.dev)), "ifn_paged_prefill_fp8");
+                  static_cast<const int32_t*>(bt.data_ptr()), small(mp), int32_t(start), N, Q, P.hkv, P.d, P.bs, scale,
+                  w.ws, w.bytes, w.stream), "ifn_paged_prefill_fp8");
   return done(out, a[7]);
 }
 
@@ -717,7 +721,7 @@ PyObject* bind(PyObject*, PyObject* args) {
 PyMethodDef methods[] = {
     IFN_FAST(decode, 16), IFN_FAST(prep_decode, 20), IFN_FAST(prefill, 11), IFN_FAST(prep_prefill, 15),
     IFN_FAST(prep_append, 13), IFN_FAST(store, 6), IFN_FAST(store_layers, 5),
-    IFN_FAST(store_fp8, 7), IFN_FAST(decode_fp8, 14), IFN_FAST(prefill_fp8, 8), IFN_FAST(evict, 8),
+    IFN_FAST(store_fp8, 7), IFN_FAST(decode_fp8, 14), IFN_FAST(prefill_fp8, 9), IFN_FAST(evict, 8),
     {"bind", bind, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast_call", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -69,10 +69,107 @@ __device__ __forceinline__ float f8_amax8(f16x8 x) {
   return m;
 }
 
+__device__ __forceinline__ float swap_max16(float x) {  // over lanes l, l ^ 16
+#if defined(__HIP_DEVICE_COMPILE__)
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+#else
+  return x;
+#endif
+}
+__device__ __forceinline__ float swap_sum(float x) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
+#if defined(__HIP_DEVICE_COMPILE__)
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(t[0]) + __uint_as_float(t[1]);
+#else
+  return x;
+#endif
+}
+
+#if defined(__HIP_DEVICE_COMPILE__)
+__device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16(f16x4 a, f16x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0);
+}
+#else
+__device__ __forceinline__ f32x4 mfma16(f16x8, f16x8, f32x4 c) { return c; }
+__device__ __forceinline__ f32x4 mfma16(f16x4, f16x4, f32x4 c) { return c; }
+#endif
+
+// One page of one head in a wave's registers, lane (n = lane % 16, g = lane / 16): K chunk i = dims 64 i + 16 g .. + 15
+// of token n, V row t = dims n D / 16 .. of token 4 g + t.  As a 16-row fragment (f8_frag) chunk i's halves are K's
+// dims in the order (i, half, g, 8 dims); a transposed V word (f8_transpose) is one dim of the lane's four tokens.
+template <int D>
+struct F8Page {
+  static constexpr int kKL = D / 64, kVW = D / 64;  // 16-byte chunks of K; words per V row
+  u32x4 k[kKL];
+  uint32_t v[4][kVW];
+};
+
+template <int D, bool kStream>
+__device__ __forceinline__ void f8_load_page(const uint8_t* k, const uint8_t* v, F8Page<D>& r) {  // the lane's addresses
+  constexpr int kVW = F8Page<D>::kVW;
+#pragma unroll
+  for (int i = 0; i < F8Page<D>::kKL; ++i) r.k[i] = kStream ? ld16_stream(k + 64 * i) : ld16(k + 64 * i);
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    if constexpr (kVW == 1) {
+      const uint32_t* p = reinterpret_cast<const uint32_t*>(v + t * D);
+      r.v[t][0] = kStream ? __builtin_nontemporal_load(p) : *p;
+    } else if constexpr (kVW == 2) {
+      const u32x2* p = reinterpret_cast<const u32x2*>(v + t * D);
+      const u32x2 x = kStream ? __builtin_nontemporal_load(p) : *p;
+      r.v[t][0] = x[0];
+      r.v[t][1] = x[1];
+    } else {
+      const u32x4 x = kStream ? ld16_stream(v + t * D) : ld16(v + t * D);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r.v[t][j % kVW] = x[j];
+    }
+  }
+}
+// Word j of tr: dim 4 c + j of the lane's V rows, one byte for each of its four tokens.
+__device__ __forceinline__ void f8_transpose4(uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3, uint32_t (&tr)[4]) {
+  const uint32_t ab = __builtin_amdgcn_perm(r1, r0, 0x05010400u), ab2 = __builtin_amdgcn_perm(r1, r0, 0x07030602u);
+  const uint32_t cd = __builtin_amdgcn_perm(r3, r2, 0x05010400u), cd2 = __builtin_amdgcn_perm(r3, r2, 0x07030602u);
+  tr[0] = __builtin_amdgcn_perm(cd, ab, 0x05040100u);
+  tr[1] = __builtin_amdgcn_perm(cd, ab, 0x07060302u);
+  tr[2] = __builtin_amdgcn_perm(cd2, ab2, 0x05040100u);
+  tr[3] = __builtin_amdgcn_perm(cd2, ab2, 0x07060302u);
+}
+template <int D>
+__device__ __forceinline__ void f8_transpose(const F8Page<D>& r, int c, uint32_t (&tr)[4]) {
+  f8_transpose4(r.v[0][c], r.v[1][c], r.v[2][c], r.v[3][c], tr);
+}
+// Eight codes (two words, a scale each) as a fragment of eight fp16.
+__device__ __forceinline__ f16x8 f8_frag(uint32_t w0, uint32_t w1, float s0, float s1) {
+  const f16x2 a = f8_to_f16<false>(w0, s0), b = f8_to_f16<true>(w0, s0), c = f8_to_f16<false>(w1, s1),
+              d = f8_to_f16<true>(w1, s1);
+  return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// No instruction: the values must have arrived at this point.
+template <class A, class B>
+__device__ __forceinline__ void settle(A& a, B& b) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" : "+v"(a));
+  asm volatile("" : "+v"(b));
+#endif
+}
+
 // Byte offset of block (page, head) in the K or V half.
 template <int D>
 __device__ __forceinline__ int64_t f8_block(int64_t page, int hkv, int h) {
   return (page * hkv + h) * (kF8Page * D);
 }
+
+// Prefill in workgroups of 128 columns (paged_prefill_fp8_block.hip), on one or two key groups.
+int prefill_fp8_block_launch(f16* out, const f16* q, const uint8_t* codes, const float* scales, int64_t num_pages,
+                             const int32_t* table, int32_t query_start, int32_t T, int32_t hq, int32_t hkv, int32_t d,
+                             float scale_log2, int groups, hipStream_t stream);
 
 }  // namespace ifn

@@ -72,55 +72,7 @@ struct F8Workspace {
   float* lse;
 };
 
-__device__ __forceinline__ float swap_max16(float x) {  // over lanes l, l ^ 16
-#if defined(__HIP_DEVICE_COMPILE__)
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-#else
-  return x;
-#endif
-}
-__device__ __forceinline__ float swap_sum(float x) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
-#if defined(__HIP_DEVICE_COMPILE__)
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-  const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(t[0]) + __uint_as_float(t[1]);
-#else
-  return x;
-#endif
-}
-
-#if defined(__HIP_DEVICE_COMPILE__)
-__device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x4 mfma16(f16x4 a, f16x4 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0);
-}
-#else
-__device__ __forceinline__ f32x4 mfma16(f16x8, f16x8, f32x4 c) { return c; }
-__device__ __forceinline__ f32x4 mfma16(f16x4, f16x4, f32x4 c) { return c; }
-#endif
-
-// One page of one head as loaded: K chunk i = 16 dims of token n, V row t = D / 16 dims of token 4 g + t.
-template <int D>
-struct F8Page {
-  static constexpr int kKL = D / 64, kVW = D / 64;  // 16-byte chunks of K; words per V row
-  u32x4 k[kKL];
-  uint32_t v[4][kVW];
-};
-
 // Pages of row b in the list: its own, and kRowStart more in front when it has any.
-// No instruction: the values must have arrived at this point.
-template <class A, class B>
-__device__ __forceinline__ void settle(A& a, B& b) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  asm volatile("" : "+v"(a));
-  asm volatile("" : "+v"(b));
-#endif
-}
-
 template <int kWaves>
 __device__ __forceinline__ int f8_offsets(int* s_cum, int* s_wsum, const int32_t* seq_lens, const uint8_t* active,
                                           int batch, int cap) {
@@ -355,23 +307,7 @@ __global__ __launch_bounds__(kDecThreads, f8_per_simd(D)) void decode_fp8_kernel
       const int raw = page_id(p), id = in_pool(raw) ? raw : 0;
       const uint8_t* kb = cache.codes + f8_block<D>(id, hkv, h);
       const uint8_t* vb = kb + v_codes;
-#pragma unroll
-      for (int i = 0; i < kKL; ++i) r.k[i] = ld16_stream(kb + k_lane + 64 * i);
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const uint8_t* p4 = vb + v_lane + t * D;
-        if constexpr (kVW == 1) {
-          r.v[t][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p4));
-        } else if constexpr (kVW == 2) {
-          const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p4));
-          r.v[t][0] = x[0];
-          r.v[t][1] = x[1];
-        } else {
-          const u32x4 x = ld16_stream(p4);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) r.v[t][j % kVW] = x[j];
-        }
-      }
+      f8_load_page<D, true>(kb + k_lane, vb + v_lane, r);
     };
     const int last = np - 1;
 
@@ -453,10 +389,7 @@ __global__ __launch_bounds__(kDecThreads, f8_per_simd(D)) void decode_fp8_kernel
       for (int c = 0; c < kKL; ++c) {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const uint32_t w0 = r.k[c][2 * half], w1 = r.k[c][2 * half + 1];
-          const f16x2 h0 = f8_to_f16<false>(w0, ks), h1 = f8_to_f16<true>(w0, ks), h2 = f8_to_f16<false>(w1, ks),
-                      h3 = f8_to_f16<true>(w1, ks);
-          s = mfma16(f16x8{h0[0], h0[1], h1[0], h1[1], h2[0], h2[1], h3[0], h3[1]}, qf[2 * c + half], s);
+          s = mfma16(f8_frag(r.k[c][2 * half], r.k[c][2 * half + 1], ks, ks), qf[2 * c + half], s);
         }
       }
       // scores in base 2; tokens past the row's end, and of pages outside the pool, have none
@@ -495,13 +428,8 @@ __global__ __launch_bounds__(kDecThreads, f8_per_simd(D)) void decode_fp8_kernel
       const f16x4 pf = f16x4{f16(pr[0]), f16(pr[1]), f16(pr[2]), f16(pr[3])};
 #pragma unroll
       for (int c = 0; c < kVW; ++c) {
-        // byte transpose: word j = dim 4 c + j of tokens 4 g .. 4 g + 3
-        const uint32_t ab = __builtin_amdgcn_perm(r.v[1][c], r.v[0][c], 0x05010400u);
-        const uint32_t ab2 = __builtin_amdgcn_perm(r.v[1][c], r.v[0][c], 0x07030602u);
-        const uint32_t cd = __builtin_amdgcn_perm(r.v[3][c], r.v[2][c], 0x05010400u);
-        const uint32_t cd2 = __builtin_amdgcn_perm(r.v[3][c], r.v[2][c], 0x07030602u);
-        const uint32_t tr[4] = {__builtin_amdgcn_perm(cd, ab, 0x05040100u), __builtin_amdgcn_perm(cd, ab, 0x07060302u),
-                                __builtin_amdgcn_perm(cd2, ab2, 0x05040100u), __builtin_amdgcn_perm(cd2, ab2, 0x07060302u)};
+        uint32_t tr[4];
+        f8_transpose(r, c, tr);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const f16x2 h0 = f8_to_f16<false>(tr[j], vs), h1 = f8_to_f16<true>(tr[j], vs);

@@ -26,7 +26,8 @@ _ENTRIES = ("ifn_store_kv", "ifn_store_kv_layers", "ifn_paged_decode_workspace_b
             "ifn_paged_prefill_workspace_bytes", "ifn_paged_prefill", "ifn_paged_prefill_append",
             "ifn_qk_norm_rope_append", "ifn_paged_decode_prep_append", "ifn_paged_decode_prep_append_planning",
             "ifn_paged_prefill_prep_append", "ifn_store_kv_fp8", "ifn_paged_decode_fp8_workspace_bytes",
-            "ifn_paged_decode_fp8", "ifn_paged_decode_append_fp8", "ifn_paged_prefill_fp8", "ifn_evict_pages")
+            "ifn_paged_decode_fp8", "ifn_paged_decode_append_fp8",
+            "ifn_paged_prefill_fp8_workspace_bytes", "ifn_paged_prefill_fp8", "ifn_evict_pages")
 
 
 def _none(*args):

@@ -252,7 +252,7 @@ def paged_attention_fp8(query: torch.Tensor, kv_pool: torch.Tensor, scales: torc
                        scale, out, max_seq_len, page_weights, validate)
     if (sequence_lengths is None and active_mask is None and max_seq_len is None and page_weights is None and
             not validate):
-        o = _fast.prefill_fp8(query, kv_pool, scales, block_tables, query_start, layer, scale, out)
+        o = _fast.prefill_fp8(query, kv_pool, scales, block_tables, query_start, layer, scale, out, _WORKSPACES)
         if o is not None:
             return o
     return _prefill(query, kv_pool, scales, block_tables, sequence_lengths, active_mask, layer, scale, query_start, out,
@@ -300,8 +300,11 @@ def _prefill(query, kv_pool, scales, block_tables, sequence_lengths, active_mask
         _validate_pages(table[None, :], keys, P, BLOCK, "paged_attention_fp8 (prefill)")
         _validate_scales(scales_layer, table[None, :], keys)
     with _current(dev):
+        stream = current_stream(dev)
+        nbytes = _capi.lib().ifn_paged_prefill_fp8_workspace_bytes(n, query_start, hq, hkv, d, BLOCK)
+        ws = _workspace(dev, stream, nbytes)
         _capi.call("ifn_paged_prefill_fp8", ptr(out), ptr(query), ptr(pool_layer), ptr(scales_layer), P, ptr(table),
-                   table.shape[0], query_start, n, hq, hkv, d, BLOCK, float(scale), current_stream(dev))
+                   table.shape[0], query_start, n, hq, hkv, d, BLOCK, float(scale), ptr(ws), ws.numel(), stream)
     return out
 
 

@@ -63,7 +63,8 @@ def test_decode_entry_points(append):
 
 def test_prefill_entry_point():
     L = _capi.lib()
-    ok = dict(out=A, q=A, c=A, s=A, P=64, bt=A, W=32, qs=0, T=16, hq=16, hkv=8, d=128, bs=16, scale=0.0)
+    ok = dict(out=A, q=A, c=A, s=A, P=64, bt=A, W=32, qs=0, T=16, hq=16, hkv=8, d=128, bs=16, scale=0.0,
+              ws=A, wsb=1 << 40)
 
     def call(**kw):
         a = {**ok, **kw}
@@ -76,6 +77,8 @@ def test_prefill_entry_point():
         assert call(**kw) == _capi.IFN_ERR_UNSUPPORTED
     assert call(out=A + 2) == _capi.IFN_ERR_ALIGNMENT
     assert call(T=0) == _capi.IFN_OK
+    assert call(ws=None) == _capi.IFN_ERR_WORKSPACE and call(wsb=64) == _capi.IFN_ERR_WORKSPACE
+    assert L.ifn_paged_prefill_fp8_workspace_bytes(16, -1, 16, 8, 128, 16) == 0
 
 
 def test_evict_entry_point():
