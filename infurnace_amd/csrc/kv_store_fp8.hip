@@ -8,10 +8,14 @@
 //   otherwise:   s' = max(s, need), and its other codes become e4m3(c s / s')  (unchanged where s' = s)
 //   c'[o_t] = e4m3(x_t / s')
 //
-// A block is changed as a whole, so one wave owns it: the wave of the call's first token in that page (a
-// token has none of its page among the 63 before it), which finds the page's other tokens among the 63 that
-// follow.  A call keeps a page's tokens that near to each other (any order; of two with one slot the later
-// is stored).  Lane (row = lane / 4, part = lane % 4) holds 8 dims of every 32 of one of the block's 16 rows.
+// A block is changed as a whole, so one wave owns a page's two blocks of a head: the wave of the call's first token in
+// that page (a token has none of its page among the 63 before it), which finds the page's other tokens among the 63
+// that follow.  A call keeps a page's tokens that near to each other (any order; of two with one slot the later
+// is stored).  D / 8 lanes take a row, 8 dims each: a load instruction reads whole rows of a head, a store writes
+// whole lines of a block.
+//
+// What bounds it: small calls by their round trips (slots, rows and scales, stores), 4.4 us; large ones by memory (8192
+// tokens of 8 x 128: 12.0 us, 4.2 TB/s; 30000: 34.6 us, 5.3 TB/s, where a large copy reaches 4.7).
 #include "kv_fp8.hpp"
 
 namespace ifn {
@@ -19,20 +23,29 @@ namespace ifn {
 constexpr int kStoreF8Threads = 256;
 constexpr int kStoreF8Waves = kStoreF8Threads / kWave;
 
+// Maximum over the 64 lanes.
+__device__ __forceinline__ float wave_max_fast(float x) {
+  x = fmaxf(x, dpp<kDppXor1>(x));
+  x = fmaxf(x, dpp<kDppXor2>(x));
+  x = fmaxf(x, dpp<kDppHalfMirror>(x));
+  x = fmaxf(x, dpp<kDppMirror>(x));
+  return max_lane32(swap_max16(x));
+}
+
 // per: consecutive tokens a wave looks at for first ones.
 template <int D>
 __global__ __launch_bounds__(kStoreF8Threads) void store_kv_fp8_kernel(
     uint8_t* __restrict__ codes, float* __restrict__ scales, int64_t num_pages, const int32_t* __restrict__ slots,
     const uint8_t* __restrict__ active, const f16* __restrict__ new_k, const f16* __restrict__ new_v,
     int32_t num_tokens, int32_t hkv, int32_t per) {
-  constexpr int kC = D / 32;  // 8-dim pieces of a row per lane
+  constexpr int kLanes = D / 8;           // lanes per row
+  constexpr int kRows = kWave / kLanes;   // rows per instruction
+  constexpr int kC = kF8Page / kRows;     // instructions per block: instruction c, rows kRows c + lane / kLanes
   const int lane = threadIdx.x % kWave;
   const int64_t w = int64_t(blockIdx.x) * kStoreF8Waves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int which = int(w % (2 * hkv));  // K heads, then V heads
-  const int64_t t0 = w / (2 * hkv) * per;
+  const int h = int(w % hkv);
+  const int64_t t0 = w / hkv * per;
   if (t0 >= num_tokens) return;
-  const bool is_v = which >= hkv;
-  const int h = is_v ? which - hkv : which;
   const int64_t num_slots = num_pages * kF8Page;
   // slots of the 64 tokens before t0, from t0 on, and after those; -1 where nothing is stored
   auto slot_at = [&](int64_t t) -> int {
@@ -43,61 +56,73 @@ __global__ __launch_bounds__(kStoreF8Threads) void store_kv_fp8_kernel(
   };
   const int s0 = slot_at(t0 - kWave + lane), s1 = slot_at(t0 + lane);
   const int s2 = per > 1 ? slot_at(t0 + kWave + lane) : -1;
-  const f16* src = (is_v ? new_v : new_k) + int64_t(h) * D;
-  const int row = lane / 4, part = lane % 4;
+  const int p0 = s0 >> 4, p1 = s1 >> 4, p2 = s2 >> 4;  // pages (-1: none)
+  // first tokens are among those whose page is not the one before's
+  int before = __shfl_up(p1, 1);
+  const int last0 = __builtin_amdgcn_readlane(p0, kWave - 1);
+  if (lane == 0) before = last0;
+  uint64_t todo = __builtin_amdgcn_ballot_w64(p1 >= 0 && p1 != before && lane < per);
+  const int row0 = lane / kLanes, piece = 8 * (lane % kLanes);
 
-  for (int i = 0; i < per; ++i) {
-    const int slot = __builtin_amdgcn_readlane(s1, i);
-    if (slot < 0) continue;
-    const int page = slot / kF8Page;
-    const bool m0 = s0 >= 0 && s0 / kF8Page == page && lane > i;  // the 63 tokens before token t0 + i
-    const bool m1 = s1 >= 0 && s1 / kF8Page == page;
-    const bool m2 = s2 >= 0 && s2 / kF8Page == page && lane < i;  // ... and up to the 63 behind it
-    if (__builtin_amdgcn_ballot_w64(m0 || (m1 && lane < i)) != 0) continue;
-    // the block's rows in this call: the latest token of each offset
-    int from = -1;
-#pragma unroll
-    for (int o = 0; o < kF8Page; ++o) {
-      const uint64_t b1 = __builtin_amdgcn_ballot_w64(m1 && s1 % kF8Page == o);
-      const uint64_t b2 = __builtin_amdgcn_ballot_w64(m2 && s2 % kF8Page == o);
-      const int f = b2 != 0 ? 127 - __builtin_clzll(b2) : b1 != 0 ? 63 - __builtin_clzll(b1) : -1;
-      if (row == o) from = f;
-    }
-    const bool mine = from >= 0;
-    const bool begins = __builtin_amdgcn_readlane(from, 0) >= 0;
-    f16x8 x[kC];
-    float amax = 0.f;
-    if (mine) {
-      const f16* p = src + (t0 + from) * hkv * D + 8 * part;
-#pragma unroll
-      for (int c = 0; c < kC; ++c) x[c] = as_h8(ld16_stream(p + 32 * c));
-    }
-    const int64_t sc = ((is_v ? num_pages : 0) + page) * hkv + h;
-    const float old = scales[sc];
-    if (mine) {
-#pragma unroll
-      for (int c = 0; c < kC; ++c) amax = fmaxf(amax, f8_amax8(x[c]));
-    }
-    amax = wave_max(amax);
-    const float need = f8_pow2(f8_need_exp(amax));
-    const float now = begins ? need : fmaxf(old, need);
-    uint8_t* blk = codes + (is_v ? num_pages * hkv * (kF8Page * D) : 0) + f8_block<D>(page, hkv, h) + row * D + 8 * part;
-    if (mine) {
-      const float inv = 1.f / now;  // (exact: a power of two)
-#pragma unroll
-      for (int c = 0; c < kC; ++c) *reinterpret_cast<u32x2*>(blk + 32 * c) = f8_quant8(x[c], inv);
-    } else if (begins) {
-#pragma unroll
-      for (int c = 0; c < kC; ++c) *reinterpret_cast<u32x2*>(blk + 32 * c) = u32x2{0u, 0u};
-    } else if (now != old) {
-      const float ratio = old / now;
+  while (todo != 0) {
+    const int i = __builtin_ctzll(todo);
+    todo &= todo - 1;
+    const int slot = __builtin_amdgcn_readlane(s1, i), page = slot >> 4;
+    const bool m1 = p1 == page;
+    const bool m2 = p2 == page && lane < i;  // (up to the 63 behind the token)
+    if (__builtin_amdgcn_ballot_w64((p0 == page && lane > i) || (m1 && lane < i)) != 0) continue;
+    // the block's rows in this call, as tokens from t0: a run of the page's tokens in order, or the latest of each offset
+    int from[kC];
+    const uint64_t b1 = __builtin_amdgcn_ballot_w64(m1), b2 = __builtin_amdgcn_ballot_w64(m2);
+    if (b2 == 0 && __builtin_amdgcn_ballot_w64(m1 && s1 - slot != lane - i) == 0) {
+      const int end = (slot & 15) + __builtin_popcountll(b1);
 #pragma unroll
       for (int c = 0; c < kC; ++c) {
-        const u32x2 v = *reinterpret_cast<const u32x2*>(blk + 32 * c);
-        *reinterpret_cast<u32x2*>(blk + 32 * c) = u32x2{f8_rescale(v[0], ratio), f8_rescale(v[1], ratio)};
+        const int row = kRows * c + row0;
+        from[c] = row >= (slot & 15) && row < end ? i + row - (slot & 15) : -1;
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < kC; ++c) from[c] = -1;
+#pragma unroll
+      for (int o = 0; o < kF8Page; ++o) {
+        const uint64_t o1 = __builtin_amdgcn_ballot_w64(m1 && (s1 & 15) == o);
+        const uint64_t o2 = __builtin_amdgcn_ballot_w64(m2 && (s2 & 15) == o);
+        const int f = o2 != 0 ? 127 - __builtin_clzll(o2) : o1 != 0 ? 63 - __builtin_clzll(o1) : -1;
+        if (row0 == o % kRows) from[o / kRows] = f;
       }
     }
-    if (lane == 0 && (begins || now != old)) scales[sc] = now;
+    const bool begins = __builtin_amdgcn_readlane(from[0], 0) >= 0;
+    f16x8 x[2][kC];
+    float old[2], amax[2] = {0.f, 0.f};
+    const int64_t src = t0 * hkv * D + int64_t(h) * D + piece;
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      const f16* rows = kv == 0 ? new_k : new_v;
+#pragma unroll
+      for (int c = 0; c < kC; ++c)  // (rows that are not in the call: zeros)
+        x[kv][c] = as_h8(from[c] >= 0 ? ld16_stream(rows + src + int64_t(from[c]) * hkv * D) : u32x4{0u, 0u, 0u, 0u});
+      old[kv] = scales[(kv * num_pages + page) * hkv + h];
+    }
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+#pragma unroll
+      for (int c = 0; c < kC; ++c) amax[kv] = fmaxf(amax[kv], f8_amax8(x[kv][c]));
+      const float need = f8_pow2(f8_need_exp(wave_max_fast(amax[kv])));
+      const float now = begins ? need : fmaxf(old[kv], need), inv = 1.f / now;  // (exact: powers of two)
+      uint8_t* blk = codes + kv * num_pages * hkv * (kF8Page * D) + f8_block<D>(page, hkv, h) + row0 * D + piece;
+#pragma unroll
+      for (int c = 0; c < kC; ++c) {
+        u32x2* dst = reinterpret_cast<u32x2*>(blk + kRows * c * D);
+        if (begins || from[c] >= 0) {  // (a block that starts: its other rows are zero)
+          *dst = f8_quant8(x[kv][c], inv);
+        } else if (now != old[kv]) {
+          const u32x2 v = *dst;
+          *dst = u32x2{f8_rescale(v[0], old[kv] / now), f8_rescale(v[1], old[kv] / now)};
+        }
+      }
+      if (lane == 0 && (begins || now != old[kv])) scales[(kv * num_pages + page) * hkv + h] = now;
+    }
   }
 }
 
@@ -119,8 +144,12 @@ extern "C" int ifn_store_kv_fp8(void* codes_layer, float* scales_layer, int64_t 
   IFN_CHECK_ALIGN16(new_k);
   IFN_CHECK_ALIGN16(new_v);
   if (num_tokens == 0) return IFN_OK;
-  const int32_t per = num_tokens >= 1024 ? kF8Page : 1;
-  const int64_t waves = ceil_div(num_tokens, per) * 2 * num_kv_heads;
+  // A wave for every token is best for the tokens of a step, each in a page of its own (8 heads, 256 of them: 5.1 us,
+  // 10.2 with four a wave, 32 with 16), a wave for every 16 for a chunk (2000 tokens: 22.4, 10.5, 5.5).  By what the
+  // call most likely is: steps have few tokens.  (512 tokens: a chunk 7.2, 5.3, 5.1, a step 6.9, 10.7, 32.9.)
+  const int64_t most = int64_t(num_tokens) * num_kv_heads;
+  const int32_t per = most <= 2048 ? 1 : most <= 8192 ? 4 : kF8Page;
+  const int64_t waves = ceil_div(num_tokens, per) * num_kv_heads;
   const int64_t blocks = ceil_div(waves, kStoreF8Waves);
   if (blocks >= int64_t(1) << 31) return IFN_ERR_UNSUPPORTED;
   const hipStream_t s = static_cast<hipStream_t>(stream);
