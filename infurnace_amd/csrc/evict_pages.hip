@@ -6,9 +6,18 @@
 // kv heads of weights[b][h][j], in 64 bits and rounded to fp32 (NaN counts as the lowest, ties go to the lower
 // j).  The row's table and weights close up in order; the evicted ids follow the kept ones.
 //
-// One workgroup per row.  The sums become integers that order as the floats do; a radix select, four passes of
-// eight bits over LDS, finds the smallest kept one and how many of its equals are kept; then one ordered pass
-// with prefix sums writes the row.  Counts are integers, so LDS atomics leave no trace of their order.
+// A row's first workgroup chooses: the sums become integers that order as the floats do; a radix select, at most three
+// passes of 11 bits over LDS, finds the smallest kept one and how many of its equals are kept; one prefix sum over the
+// threads, each with a run of the row's pages, gives every page its place, and the row is written through that
+// permutation.  Further workgroups, one per kv head, write what no choice is needed for: the zeros behind the kept
+// weights, or all the weights of a row that is not cut.  Counts are integers, so LDS atomics leave no trace of their
+// order.
+//
+// What bounds it: latency -- lengths, sums, up to three passes, the scan, the row, one after the other.  32 rows of 8-256
+// pages, 8 heads: 7.5 us (ranking by counting instead of the passes: 8.8-9.8); 64 rows of 1250-4096 pages (17 MB read and
+// written): 13.5 us, where one workgroup a row that also wrote the zeros took 24.
+#include <algorithm>
+
 #include "ifn_common.hpp"
 
 namespace ifn {
@@ -24,124 +33,153 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   return (b & 0x80000000u) != 0 ? ~b : b | 0x80000000u;
 }
 
+constexpr int kEvictBits = 11;   // of a digit
+constexpr int kEvictBins = 1 << kEvictBits;
+
+// Exclusive prefix sum of x over the workgroup's threads, and the total (s_sum: one word per wave; two barriers).
+__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* s_sum, uint32_t& total) {
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  uint32_t y = x;
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const uint32_t z = __shfl_up(y, o);
+    if (lane >= o) y += z;
+  }
+  if (lane == kWave - 1) s_sum[wave] = y;
+  __syncthreads();
+  uint32_t pre = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kEvictWaves; ++w) {
+    const uint32_t v = s_sum[w];
+    pre += w < wave ? v : 0u;
+    total += v;
+  }
+  __syncthreads();
+  return pre + y - x;
+}
+
 __global__ __launch_bounds__(kEvictThreads) void evict_pages_kernel(
     int32_t* __restrict__ out_tables, int32_t* __restrict__ out_lens, float* __restrict__ out_weights,
     int32_t* __restrict__ num_evicted, const int32_t* __restrict__ tables, int32_t max_pages,
     const int32_t* __restrict__ lens, const uint8_t* __restrict__ active, const float* __restrict__ weights,
     int32_t hkv, int32_t keep, int32_t sink, int32_t recent) {
-  extern __shared__ uint32_t s_key[];  // max_pages
-  __shared__ int s_hist[256];
-  __shared__ int s_sum[2][kEvictWaves];
-  __shared__ int s_pick[2];
-  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  extern __shared__ uint32_t s_key[];  // max_pages: the keys, then the row's permutation
+  __shared__ int s_hist[kEvictBins];
+  __shared__ uint32_t s_sum[kEvictWaves];
+  __shared__ int s_pick[3];
+  const int tid = threadIdx.x;
   const int64_t b = blockIdx.x;
-  const int cap = max_pages * 16;
   const int len = lens[b];
   const bool on = active == nullptr || active[b] != 0;
-  const int n = (max(0, min(len, cap)) + 15) / 16;
+  const int n = (max(0, min(len, max_pages * 16)) + 15) / 16;
   const bool cut = on && n > keep;
+  const float* w = weights + b * hkv * max_pages;
+  float* out_w = out_weights + b * hkv * max_pages;
+  if (blockIdx.y > 0) {
+    for (int h = int(blockIdx.y) - 1; h < hkv; h += int(gridDim.y) - 1) {
+      const int64_t at = int64_t(h) * max_pages;
+      for (int j = (cut ? keep : 0) + tid; j < max_pages; j += kEvictThreads) out_w[at + j] = !cut && j < n ? w[at + j] : 0.f;
+    }
+    return;
+  }
   const int gone = cut ? n - keep : 0;
   const int32_t* row = tables + b * max_pages;
   int32_t* out_row = out_tables + b * max_pages;
-  const float* w = weights + b * hkv * max_pages;
-  float* out_w = out_weights + b * hkv * max_pages;
   if (tid == 0) {
     out_lens[b] = len - 16 * gone;
     num_evicted[b] = gone;
   }
-  if (!cut) {
-    for (int j = tid; j < max_pages; j += kEvictThreads) out_row[j] = row[j];
-    for (int64_t i = tid; i < int64_t(hkv) * max_pages; i += kEvictThreads)
-      out_w[i] = int(i % max_pages) < n ? w[i] : 0.f;
-    return;
+  for (int j = (cut ? n : 0) + tid; j < max_pages; j += kEvictThreads) out_row[j] = row[j];
+  if (!cut) return;
+
+  // keys of the candidates [lo, hi): four pages of eight heads a thread are in flight
+  const int lo = sink, hi = n - recent;
+  for (int j0 = lo; j0 < hi; j0 += 4 * kEvictThreads) {
+    double sum[4] = {0.0, 0.0, 0.0, 0.0};
+    for (int h0 = 0; h0 < hkv; h0 += 8) {
+      float v[4][8];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int j = min(j0 + c * kEvictThreads + tid, hi - 1);
+        if (j0 + c * kEvictThreads >= hi) continue;  // (uniform)
+#pragma unroll
+        for (int x = 0; x < 8; ++x) v[c][x] = w[int64_t(min(h0 + x, hkv - 1)) * max_pages + j];
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if (j0 + c * kEvictThreads >= hi) continue;
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+          if (h0 + x < hkv) sum[c] += double(v[c][x]);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int j = j0 + c * kEvictThreads + tid;
+      if (j < hi) s_key[j] = order_key(float(sum[c]));
+    }
   }
-  const int lo = sink, hi = n - recent;  // candidates [lo, hi)
-  for (int j = lo + tid; j < hi; j += kEvictThreads) {
-    double s = 0.0;
-    for (int h = 0; h < hkv; ++h) s += double(w[int64_t(h) * max_pages + j]);
-    s_key[j] = order_key(float(s));
-  }
-  // the left-th largest key, digit by digit
+  // the left-th largest key, digit by digit; left: how many of those equal to it (under mask) are kept
   int left = keep - sink - recent;
   uint32_t prefix = 0, mask = 0;
-  if (left > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) s_hist[tid] = 0;
-      __syncthreads();
-      for (int j = lo + tid; j < hi; j += kEvictThreads) {
-        const uint32_t k = s_key[j];
-        if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & 255u], 1);
-      }
-      __syncthreads();
-      if (wave == 0) {  // lane i: digits 255 - 4 i .. 252 - 4 i
-        int c[4], mine = 0;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) mine += c[x] = s_hist[255 - 4 * lane - x];
-        int upto = mine;
-#pragma unroll
-        for (int o = 1; o < kWave; o <<= 1) {
-          const int y = __shfl_up(upto, o);
-          if (lane >= o) upto += y;
-        }
-        int before = upto - mine;
-        if (before < left && upto >= left) {
-          int x = 0;
-          while (before + c[x] < left) before += c[x++];
-          s_pick[0] = 255 - 4 * lane - x;
-          s_pick[1] = left - before;
-        }
-      }
-      __syncthreads();
-      prefix |= uint32_t(s_pick[0]) << shift;
-      mask |= 255u << shift;
-      left = s_pick[1];
-    }
-  } else {
+  for (int shift = 32 - kEvictBits; left > 0; shift = max(shift - kEvictBits, 0)) {
+    const uint32_t digit = shift == 0 ? ~mask : uint32_t(kEvictBins - 1) << shift;
+    s_hist[tid] = 0;
+    s_hist[tid + kEvictThreads] = 0;
     __syncthreads();
-  }
-  // kept: over the key, or one of the first `left` equal to it
-  int kept = 0, equal = 0;
-  for (int j0 = 0; j0 < max_pages; j0 += kEvictThreads) {
-    const int j = j0 + tid;
-    bool eq = false, take = j < lo || (j >= hi && j < n);
-    if (j >= lo && j < hi && keep > sink + recent) {
+    for (int j = lo + tid; j < hi; j += kEvictThreads) {
       const uint32_t k = s_key[j];
-      take = k > prefix;
-      eq = k == prefix;
+      if ((k & mask) == prefix) atomicAdd(&s_hist[(k & digit) >> shift], 1);
     }
-    const uint64_t beq = __builtin_amdgcn_ballot_w64(eq);
-    if (lane == 0) s_sum[0][wave] = __builtin_popcountll(beq);
     __syncthreads();
-    int pre = 0, tot = 0;
-#pragma unroll
-    for (int x = 0; x < kEvictWaves; ++x) {
-      const int v = s_sum[0][x];
-      pre += x < wave ? v : 0;
-      tot += v;
+    // thread i: bins 2047 - 2 i and 2046 - 2 i
+    const int c0 = s_hist[kEvictBins - 1 - 2 * tid], c1 = s_hist[kEvictBins - 2 - 2 * tid];
+    uint32_t total;
+    const int before = int(block_scan(uint32_t(c0 + c1), s_sum, total));
+    if (before < left && before + c0 + c1 >= left) {  // (one thread)
+      const bool second = before + c0 < left;
+      s_pick[0] = kEvictBins - 1 - 2 * tid - (second ? 1 : 0);
+      s_pick[1] = left - before - (second ? c0 : 0);
+      s_pick[2] = second ? c1 : c0;
     }
-    const uint64_t below = (uint64_t(1) << lane) - 1;
-    if (eq && equal + pre + __builtin_popcountll(beq & below) < left) take = true;
-    equal += tot;
-    const uint64_t bt = __builtin_amdgcn_ballot_w64(take);
-    if (lane == 0) s_sum[1][wave] = __builtin_popcountll(bt);
     __syncthreads();
-    pre = tot = 0;
-#pragma unroll
-    for (int x = 0; x < kEvictWaves; ++x) {
-      const int v = s_sum[1][x];
-      pre += x < wave ? v : 0;
-      tot += v;
+    prefix |= uint32_t(s_pick[0]) << shift;
+    mask |= digit;
+    left = s_pick[1];
+    if (shift == 0 || left == s_pick[2]) break;  // (all of the bin's are kept: its lower digits do not matter)
+  }
+  // Each thread: a run of `per` pages.  Kept: over the key, or one of the first `left` equal to it.
+  const int per = (n + kEvictThreads - 1) / kEvictThreads, first = tid * per;  // (per <= 32)
+  uint32_t over = 0, same = 0;
+  for (int k = 0; k < per; ++k) {
+    const int j = first + k;
+    if (j >= n) break;
+    if (j < lo || j >= hi) {
+      over |= 1u << k;
+    } else if (left > 0) {
+      const uint32_t key = s_key[j] & mask;
+      over |= uint32_t(key > prefix) << k;
+      same |= uint32_t(key == prefix) << k;
     }
-    const int at = kept + pre + __builtin_popcountll(bt & below);  // kept pages before j
-    kept += tot;
-    if (j < max_pages) {
-      const int dst = j >= n ? j : take ? at : keep + j - at;
-      out_row[dst] = row[j];
-      for (int h = 0; h < hkv; ++h) {
-        const int64_t base = int64_t(h) * max_pages;
-        out_w[base + dst] = take ? w[base + j] : 0.f;
-      }
-    }
+  }
+  uint32_t total;
+  const uint32_t before = block_scan(uint32_t(__popc(over)) << 16 | uint32_t(__popc(same)), s_sum, total);
+  int over_before = int(before >> 16), same_before = int(before & 0xffffu);
+  for (int k = 0; k < per; ++k) {  // (every key has been read: the scan's barriers)
+    const int j = first + k;
+    if (j >= n) break;
+    const bool s = (same >> k) & 1u, take = ((over >> k) & 1u) != 0 || (s && same_before < left);
+    const int at = over_before + min(same_before, left);  // kept pages before j
+    s_key[take ? at : keep + j - at] = uint32_t(j);
+    over_before += (over >> k) & 1u;
+    same_before += s ? 1 : 0;
+  }
+  __syncthreads();
+  for (int j = tid; j < n; j += kEvictThreads) out_row[j] = row[s_key[j]];
+  for (int x = tid; x < keep * hkv; x += kEvictThreads) {
+    const int64_t at = int64_t(x / keep) * max_pages;
+    out_w[at + x % keep] = w[at + s_key[x % keep]];
   }
 }
 
@@ -159,9 +197,11 @@ extern "C" int ifn_evict_pages(int32_t* out_tables, int32_t* out_lens, float* ou
   if (batch < 0 || max_pages_per_seq < 1 || num_kv_heads < 1 || block_size < 1 || sink_pages < 0 || recent_pages < 1 ||
       int64_t(keep_pages) < int64_t(sink_pages) + recent_pages)
     return IFN_ERR_INVALID_ARGUMENT;
-  if (block_size != 16 || max_pages_per_seq > kEvictMaxPages) return IFN_ERR_UNSUPPORTED;
+  if (block_size != 16 || max_pages_per_seq > kEvictMaxPages ||
+      int64_t(std::min(keep_pages, max_pages_per_seq)) * num_kv_heads >= int64_t(1) << 31)
+    return IFN_ERR_UNSUPPORTED;
   if (batch == 0) return IFN_OK;
-  evict_pages_kernel<<<dim3(unsigned(batch)), dim3(kEvictThreads), size_t(max_pages_per_seq) * 4,
+  evict_pages_kernel<<<dim3(unsigned(batch), unsigned(1 + std::min<int32_t>(num_kv_heads, 32))), dim3(kEvictThreads), size_t(max_pages_per_seq) * 4,
                        static_cast<hipStream_t>(stream)>>>(
       out_tables, out_lens, out_weights, num_evicted, block_tables, max_pages_per_seq, seq_lens, active_mask,
       page_weights, num_kv_heads, keep_pages, sink_pages, recent_pages);
