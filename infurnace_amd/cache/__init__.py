@@ -5,9 +5,9 @@ docs/roadmap.md:325-337 and docs/architecture.md:225-240, 255-257.
 """
 from .block_pool import (OWNERS, BlockPool, BlockPoolError, PoolExhausted, build_block_table, slot_mapping,
                          slot_mapping_for_positions)
-from .kv_manager import KVCacheError, KVManager, PagedKVCache
+from .kv_manager import KVCacheError, KVManager, PagedKVCache, PagedKVCacheFP8
 from .prefix_cache import PrefixCache, PrefixCacheError
 
 __all__ = ["BlockPool", "BlockPoolError", "PoolExhausted", "OWNERS", "build_block_table", "slot_mapping",
-           "slot_mapping_for_positions", "KVManager", "PagedKVCache", "KVCacheError", "PrefixCache",
+           "slot_mapping_for_positions", "KVManager", "PagedKVCache", "PagedKVCacheFP8", "KVCacheError", "PrefixCache",
            "PrefixCacheError"]

@@ -20,7 +20,7 @@ import torch
 
 from .block_pool import BlockPool, BlockPoolError, PoolExhausted, build_block_table
 
-__all__ = ["PagedKVCache", "KVManager", "KVCacheError"]
+__all__ = ["PagedKVCache", "PagedKVCacheFP8", "KVManager", "KVCacheError"]
 
 
 class KVCacheError(ValueError):
@@ -82,6 +82,80 @@ class PagedKVCache:
         from ..kernels import copy_pages
         copy_pages(self.kv, torch.as_tensor(s.astype(np.int32), device=self.kv.device),
                    torch.as_tensor(d.astype(np.int32), device=self.kv.device))
+
+
+class PagedKVCacheFP8:
+    """Persistent 8-bit cache on one GPU: ``kv`` float8_e4m3fn [layers, 2, num_blocks, num_kv_heads, 16, head_dim] and
+    ``scales`` fp32 [layers, 2, num_blocks, num_kv_heads], a power of two for each page and head (see
+    ``infurnace_amd.kernels.store_kv_fp8``).  Half the bytes of ``PagedKVCache``."""
+
+    def __init__(self, num_layers: int, num_blocks: int, num_kv_heads: int, head_dim: int, block_size: int = 16,
+                 device: str | torch.device = "cuda"):
+        for name, v in (("num_layers", num_layers), ("num_blocks", num_blocks), ("num_kv_heads", num_kv_heads)):
+            if v < 1:
+                raise KVCacheError(f"{name} must be positive, got {v}")
+        if block_size != 16:
+            raise KVCacheError(f"the 8-bit cache has 16-token pages, got block_size {block_size}")
+        if head_dim not in (64, 128, 256):
+            raise KVCacheError(f"the 8-bit cache takes head_dim 64, 128 or 256, got {head_dim}")
+        self.kv = torch.zeros((num_layers, 2, num_blocks, num_kv_heads, block_size, head_dim), dtype=torch.uint8,
+                              device=device).view(torch.float8_e4m3fn)
+        self.scales = torch.full((num_layers, 2, num_blocks, num_kv_heads), self._empty(), device=device)
+        self.num_layers, self.num_blocks, self.block_size = num_layers, num_blocks, block_size
+        self.num_kv_heads, self.head_dim = num_kv_heads, head_dim
+
+    @staticmethod
+    def _empty() -> float:
+        from ..kernels.kv_fp8 import EMPTY_SCALE
+        return EMPTY_SCALE
+
+    @property
+    def shape(self) -> tuple[int, ...]:
+        return tuple(self.kv.shape)
+
+    @property
+    def size_bytes(self) -> int:
+        return self.kv.numel() + self.scales.numel() * 4
+
+    @property
+    def page_bytes(self) -> int:
+        """Bytes of one page (K+V, all kv heads, their scales) in one layer."""
+        return 2 * self.num_kv_heads * (self.block_size * self.head_dim + 4)
+
+    def layer(self, i: int) -> tuple[torch.Tensor, torch.Tensor]:
+        return self.kv[i], self.scales[i]
+
+    def _ids(self, ids: Sequence[int]) -> torch.Tensor:
+        arr = np.asarray(ids, np.int64)
+        if int(arr.min()) < 0 or int(arr.max()) >= self.num_blocks:
+            raise KVCacheError("page id outside the pool")
+        return torch.as_tensor(arr.astype(np.int32), device=self.kv.device)
+
+    def clear_pages(self, ids: Sequence[int]) -> None:
+        """Return the given pages to the freshly allocated state in every layer."""
+        if len(ids) == 0:
+            return
+        t = self._ids(ids)
+        from ..kernels import zero_pages
+        zero_pages(self.kv.view(torch.float16), t)  # (the same pages as bytes)
+        self.scales.index_fill_(2, t.long(), self._empty())
+
+    def copy_pages(self, src: Sequence[int], dst: Sequence[int]) -> None:
+        """Copy page src[i] to dst[i] in every layer, with its scales."""
+        if len(src) != len(dst):
+            raise KVCacheError("copy_pages needs as many destinations as sources")
+        if len(src) == 0:
+            return
+        s, d = self._ids(src), self._ids(dst)
+        from ..kernels import copy_pages
+        copy_pages(self.kv.view(torch.float16), s, d)
+        self.scales[:, :, d.long()] = self.scales[:, :, s.long()]
+
+    def values(self, layer: int, ids: Sequence[int]) -> torch.Tensor:
+        """The values of the given pages as an fp16 pool's [2, pages, 16, num_kv_heads, head_dim] (exact)."""
+        t = self._ids(ids).long() if len(ids) else torch.zeros(0, dtype=torch.long, device=self.kv.device)
+        codes = self.kv[layer].view(torch.uint8)[:, t].view(torch.float8_e4m3fn).float()
+        return (codes * self.scales[layer][:, t][..., None, None]).half().transpose(2, 3).contiguous()
 
 
 @dataclass
@@ -187,6 +261,24 @@ class KVManager:
             s.blocks[i] = b
         self.pool.free(old, owner="active")
         return fresh
+
+    def evict_blocks(self, seq_id: Hashable, block_indices: Sequence[int]) -> list[int]:
+        """Drop whole pages from a sequence, wherever they are; returns pages that became free.
+
+        The sequence gets that many pages and ``block_size`` tokens each shorter, its later pages move up in its
+        table.  The page that the next token goes to, or that is not full, cannot be dropped.  A borrowed prefix
+        page only loses this sequence's reference.
+        """
+        s = self._get(seq_id)
+        idx = sorted({int(i) for i in block_indices})
+        if len(idx) != len(block_indices) or (idx and (idx[0] < 0 or idx[-1] >= s.length // self.block_size)):
+            raise KVCacheError("block indices must be distinct full pages of the sequence")
+        gone = set(idx)
+        ids = [s.blocks[i] for i in idx]
+        s.blocks = [b for i, b in enumerate(s.blocks) if i not in gone]
+        s.length -= len(idx) * self.block_size
+        s.shared -= sum(i < s.shared for i in idx)
+        return self.pool.free(ids, owner="active")
 
     # ---- tables ------------------------------------------------------------------
     def block_tables(self, seq_ids: Sequence[Hashable], max_pages: int | None = None) -> np.ndarray:

@@ -37,6 +37,9 @@ this package's pool, tables and kernels:
   shared_prefix_pages=...)``) when they are at least ``shared_prefix_min_pages``;
   a batch whose rows share pages otherwise keeps its page loads cached (an empty
   ``shared_prefix_pages``), since the default decode streams every page once.
+* ``kv_dtype="float8_e4m3fn"`` holds the K/V in 8 bits (``PagedKVCacheFP8``); with ``track_page_weights`` the
+  decode steps also add up each page's attention weight per slot, over all layers, and ``evict`` cuts long
+  sequences to the pages of most weight (``evict_pages``).
 
 The model itself (projections, MLP, logits) stays with the caller.
 """
@@ -49,9 +52,10 @@ from typing import Sequence
 import numpy as np
 import torch
 
-from .cache import BlockPool, KVCacheError, KVManager, PagedKVCache, PoolExhausted, PrefixCache
-from .kernels import (decode_plan, paged_attention, qk_norm_rope_append, qk_norm_rope_store_and_decode, store_kv,
-                      store_kv_and_decode, store_kv_and_prefill)
+from .cache import BlockPool, KVCacheError, KVManager, PagedKVCache, PagedKVCacheFP8, PoolExhausted, PrefixCache
+from .kernels import (decode_plan, evict_pages, paged_attention, paged_attention_fp8, qk_norm_rope_append,
+                      qk_norm_rope_store_and_decode, store_kv, store_kv_and_decode, store_kv_and_prefill, store_kv_fp8,
+                      store_kv_fp8_and_decode)
 
 __all__ = ["PagedKVRunner", "RunnerError"]
 
@@ -77,6 +81,10 @@ class _Step:
     event: object | None = None       # recorded after the step's latest launch
     closed: bool = False              # no further launch will be recorded
     plan: object | None = None        # decode step plan, built at the first layer
+    weights: torch.Tensor | None = None  # fp32 [B, Hkv, max_pages]: the step's page weights, over its layers
+    weight_slots: torch.Tensor | None = None  # int64 slots of the live rows they go to ...
+    weight_rows: torch.Tensor | None = None   # ... and those rows
+    staged: torch.Tensor | None = None   # fp16 K/V rows of a step from fp32 projections, for the 8-bit cache
 
     def _launched(self) -> None:
         """Record the step's completion event after a launch on the current stream."""
@@ -101,7 +109,9 @@ class _Step:
         if self.closed:
             raise RunnerError("this step is closed: a later step has begun")
         kv = self.runner.cache.kv
-        if self.query_start is not None:
+        if self.runner.fp8:
+            o = self._store_attend_fp8(layer, q, k, v, out)
+        elif self.query_start is not None:
             o = store_kv_and_prefill(q, kv, self.block_tables, k, v, query_start=self.query_start, layer=layer,
                                      out=out)
         elif self.shared_prefix is None:
@@ -115,6 +125,16 @@ class _Step:
         self._launched()
         return o
 
+    def _store_attend_fp8(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                          out: torch.Tensor | None) -> torch.Tensor:
+        kv, scales = self.runner.cache.kv, self.runner.cache.scales
+        if self.query_start is None:
+            return store_kv_fp8_and_decode(q, kv, scales, self.block_tables, self.seq_lens, self.active, k, v, layer=layer,
+                                           max_seq_len=self.max_len, out=out, page_weights=self.weights)
+        store_kv_fp8(kv, scales, self.slot_mapping, None, k, v, layer=layer)
+        return paged_attention_fp8(q, kv, scales, self.block_tables, None, layer=layer, query_start=self.query_start,
+                                   out=out)
+
     def prep_store_attend(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                           q_norm_weight: torch.Tensor, k_norm_weight: torch.Tensor, rope: torch.Tensor,
                           eps: float = 1e-6, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -126,6 +146,19 @@ class _Step:
         if self.closed:
             raise RunnerError("this step is closed: a later step has begun")
         kv = self.runner.cache.kv
+        if self.runner.fp8:  # the prepared rows go through fp16 ones, slot t for token t, to the 8-bit cache
+            t = q.shape[0]
+            if self.staged is None:
+                c = self.runner.cache
+                self.staged = torch.empty((2, -(-t // self.runner.block_size), self.runner.block_size, c.num_kv_heads,
+                                           c.head_dim), dtype=torch.float16, device=self.runner.device)
+            q16 = qk_norm_rope_append(q, k, v, q_norm_weight, k_norm_weight, rope, self.positions,
+                                      torch.arange(t, dtype=torch.int32, device=self.runner.device), self.active,
+                                      self.staged, eps=eps)
+            rows = self.staged.flatten(1, 2)[:, :t]
+            o = self._store_attend_fp8(layer, q16, rows[0], rows[1], out)
+            self._launched()
+            return o
         if self.query_start is None and self.shared_prefix is None:
             o = qk_norm_rope_store_and_decode(q, k, v, q_norm_weight, k_norm_weight, rope, self.positions,
                                               self.slot_mapping, self.active, kv, self.block_tables, self.seq_lens,
@@ -151,14 +184,25 @@ class PagedKVRunner:
     def __init__(self, num_layers: int, num_slots: int, max_context: int, num_kv_heads: int, head_dim: int,
                  num_blocks: int, device: str | torch.device = "cuda", block_size: int = 16,
                  prefix_namespace=None, prefix_capacity_blocks: int | None = None,
-                 shared_prefix_min_pages: int = 64, event_factory=None):
+                 shared_prefix_min_pages: int = 64, event_factory=None, kv_dtype: str = "float16",
+                 track_page_weights: bool = False):
+        if kv_dtype not in ("float16", "float8_e4m3fn"):
+            raise RunnerError(f"kv_dtype must be float16 or float8_e4m3fn, got {kv_dtype!r}")
+        self.fp8 = kv_dtype == "float8_e4m3fn"
+        if track_page_weights and not self.fp8:
+            raise RunnerError("page weights are gathered by the 8-bit cache's decode (kv_dtype='float8_e4m3fn')")
         if num_slots < 1 or max_context < 1:
             raise RunnerError("num_slots and max_context must be positive")
         self._num_slots, self._max_context = num_slots, max_context
         self.block_size = block_size
         self.max_pages = math.ceil(max_context / block_size)
         self.device = torch.device(device)
-        self.cache = PagedKVCache(num_layers, num_blocks, num_kv_heads, head_dim, block_size, self.device)
+        self.cache = (PagedKVCacheFP8 if self.fp8 else PagedKVCache)(num_layers, num_blocks, num_kv_heads, head_dim,
+                                                                     block_size, self.device)
+        # attention weight of each slot's pages, over its decode steps and their layers
+        self.page_weights = (torch.zeros((num_slots, num_kv_heads, self.max_pages), device=self.device)
+                             if track_page_weights else None)
+        self._evicted: dict[int, int] = {}  # tokens whose K/V were evicted, by slot
         self.pool = BlockPool(num_blocks, block_size)
         self.mgr = KVManager(self.pool, max_pages_per_seq=self.max_pages)
         # prefix cache (docs/roadmap.md:442-470) when a namespace -- checkpoint and KV-affecting
@@ -192,6 +236,10 @@ class PagedKVRunner:
         """Tokens whose K/V the slot holds."""
         return self.mgr.length(slot) if slot in self.mgr else 0
 
+    def position(self, slot: int) -> int:
+        """The slot's next position: the tokens it holds and those that were evicted."""
+        return self.length(slot) + self._evicted.get(slot, 0)
+
     def _table(self, slots: Sequence[int]) -> np.ndarray:
         pad = self.pool.dummy_block if self.pool.dummy_block is not None else 0
         t = np.full((len(slots), self.max_pages), pad, np.int32)
@@ -215,19 +263,20 @@ class PagedKVRunner:
         self._check_slot(slot)
         if num_tokens < 1:
             raise RunnerError("a prefill chunk needs at least one token")
-        if start_position != self.length(slot):
-            raise RunnerError(f"slot {slot} holds {self.length(slot)} tokens; chunk starts at {start_position}")
+        if start_position != self.position(slot):
+            raise RunnerError(f"slot {slot} holds {self.position(slot)} tokens; chunk starts at {start_position}")
         if start_position + num_tokens > self._max_context:
             raise RunnerError(f"chunk ends at {start_position + num_tokens} > max_context {self._max_context}")
         self._close_steps()
         if slot not in self.mgr:
             self.mgr.add_sequence(slot)
+        first = self.length(slot)  # (behind start_position by what was evicted)
         slots = self._reserve(lambda: self.mgr.append(slot, num_tokens))
         pos = np.arange(start_position, start_position + num_tokens, dtype=np.int32)
         table = self._table([slot])[0]
-        used = table[:-(-(start_position + num_tokens) // self.block_size)]
+        used = table[:-(-(first + num_tokens) // self.block_size)]
         return self._submit(_Step(self, self._dev(slots.astype(np.int32)), self._dev(table), None, None,
-                                  self._dev(pos), start_position, start_position + num_tokens), used)
+                                  self._dev(pos), first, first + num_tokens), used)
 
     def attach_prefix(self, slot: int, token_ids: Sequence[int]) -> int:
         """Start an empty slot from the longest cached prefix of ``token_ids`` (complete blocks).
@@ -250,6 +299,8 @@ class PagedKVRunner:
         self._check_slot(slot)
         if self.prefix is None:
             raise RunnerError("this runner has no prefix cache (prefix_namespace was not given)")
+        if self._evicted.get(slot):
+            raise RunnerError(f"slot {slot} has evicted pages: its pages are no prefix of its tokens")
         if len(token_ids) > self.length(slot):
             raise RunnerError(f"slot {slot} holds {self.length(slot)} tokens, not {len(token_ids)}")
         return self.prefix.insert(list(token_ids), self.mgr.blocks(slot))
@@ -272,8 +323,8 @@ class PagedKVRunner:
         live = [i for i, a in enumerate(active) if a]
         for i in live:
             self._check_slot(slots[i])
-            if slots[i] not in self.mgr or positions[i] != self.length(slots[i]):
-                raise RunnerError(f"row {i}: slot {slots[i]} holds {self.length(slots[i])} tokens, "
+            if slots[i] not in self.mgr or positions[i] != self.position(slots[i]):
+                raise RunnerError(f"row {i}: slot {slots[i]} holds {self.position(slots[i])} tokens, "
                                   f"decode writes position {positions[i]}")
             if positions[i] + 1 > self._max_context:
                 raise RunnerError(f"row {i}: position {positions[i]} is past max_context")
@@ -286,21 +337,27 @@ class PagedKVRunner:
             sm[i] = int(new_slots[j][0])
         lens = np.zeros(len(slots), np.int32)
         for i in live:
-            lens[i] = positions[i] + 1
+            lens[i] = self.length(slots[i])
         act = np.asarray(active, np.uint8)
         table = self._table(slots)
-        shared = self._common_pages(table[live], lens[live])
-        if len(shared) >= self.shared_prefix_min_pages:
+        # (the 8-bit decode attends every row on its own)
+        shared = self._common_pages(table[live], lens[live]) if not self.fp8 else np.zeros(0, np.int32)
+        if self.fp8:
+            prefix = None
+        elif len(shared) >= self.shared_prefix_min_pages:
             prefix = self._dev(shared)
         elif self._any_shared(table[live], lens[live]):
             prefix = self._dev(np.zeros(0, np.int32))
         else:
             prefix = None
         used = [table[i, :-(-int(lens[i]) // self.block_size)] for i in live]
-        return self._submit(_Step(self, self._dev(sm), self._dev(table), self._dev(lens), self._dev(act),
-                                  self._dev(np.asarray(positions, np.int32)), None,
-                                  int(lens.max()) if len(lens) else 0, prefix),
-                            np.concatenate(used) if used else np.zeros(0, np.int32))
+        step = _Step(self, self._dev(sm), self._dev(table), self._dev(lens), self._dev(act),
+                     self._dev(np.asarray(positions, np.int32)), None, int(lens.max()) if len(lens) else 0, prefix)
+        if self.page_weights is not None and live:
+            step.weights = torch.zeros((len(slots), *self.page_weights.shape[1:]), device=self.device)
+            step.weight_slots = self._dev(np.asarray([slots[i] for i in live], np.int64))
+            step.weight_rows = self._dev(np.asarray(live, np.int64))
+        return self._submit(step, np.concatenate(used) if used else np.zeros(0, np.int32))
 
     def _common_pages(self, table: np.ndarray, lens: np.ndarray) -> np.ndarray:
         """Leading page ids that every row of ``table`` holds at the same columns (at least two
@@ -332,7 +389,10 @@ class PagedKVRunner:
         if slot not in self.mgr:
             return []
         for st in self._inflight:  # the engine clears slots between steps: no step takes more launches
-            st.closed = True
+            self._close(st)
+        if self.page_weights is not None:
+            self.page_weights[slot].zero_()
+        self._evicted.pop(slot, None)
         owned = self.mgr.blocks(slot)
         freed = self.mgr.free_sequence(slot)
         if zero:
@@ -340,6 +400,43 @@ class PagedKVRunner:
                 self.cache.clear_pages(freed)
             held = set(owned) - set(freed)
             self._zero_on_release.update(p for p in held if self.pool.refcount(p, "inflight") > 0)
+        return freed + self.reclaim()
+
+    def evict(self, keep_pages: int, sink_pages: int = 1, recent_pages: int = 1,
+              slots: Sequence[int] | None = None) -> list[int]:
+        """Cut every slot (of ``slots``) of more than ``keep_pages`` pages to that many, by the attention weight its
+        pages have gathered (``evict_pages``); returns the pages that returned to the free pool now.
+
+        All layers lose the same pages.  Later tokens keep their positions: a slot's next one is ``position(slot)``.
+        Closes the current step and waits for its work (the choice is read back).
+        """
+        if self.page_weights is None:
+            raise RunnerError("this runner gathers no page weights (track_page_weights was not given)")
+        if sink_pages < 0 or recent_pages < 1 or keep_pages < sink_pages + recent_pages:
+            raise RunnerError(f"keep_pages {keep_pages} must hold sink_pages {sink_pages} (>= 0) and recent_pages "
+                              f"{recent_pages} (>= 1)")
+        chosen = list(range(self._num_slots)) if slots is None else list(slots)
+        for s in chosen:
+            self._check_slot(s)
+        if len(set(chosen)) != len(chosen):
+            raise RunnerError("a slot is listed twice")
+        self._close_steps()
+        chosen = [s for s in chosen if s in self.mgr and len(self.mgr.blocks(s)) > keep_pages]
+        if not chosen:
+            return []
+        rows = self._dev(np.asarray(chosen, np.int64))
+        table, _, weights, gone = evict_pages(self._dev(self._table(chosen)), self._dev(self.mgr.seq_lens(chosen)),
+                                              self.page_weights[rows], keep_pages, sink_pages=sink_pages,
+                                              recent_pages=recent_pages)
+        self.page_weights[rows] = weights
+        table, gone = table.cpu().numpy(), gone.cpu().numpy()
+        freed: list[int] = []
+        for i, s in enumerate(chosen):
+            blocks = self.mgr.blocks(s)
+            kept = len(blocks) - int(gone[i])
+            out = set(table[i, kept:len(blocks)].tolist())
+            freed += self.mgr.evict_blocks(s, [j for j, p in enumerate(blocks) if p in out])
+            self._evicted[s] = self._evicted.get(s, 0) + int(gone[i]) * self.block_size
         return freed + self.reclaim()
 
     # -- in-flight pages ----------------------------------------------------------------------
@@ -358,8 +455,15 @@ class PagedKVRunner:
     def _close_steps(self) -> None:
         """A new step begins: earlier steps take no further launches; release what has completed."""
         for st in self._inflight:
-            st.closed = True
+            self._close(st)
         self.reclaim()
+
+    def _close(self, step: _Step) -> None:
+        """No launch follows in the step: its page weights go to its slots'."""
+        if not step.closed and step.weights is not None:
+            self.page_weights.index_add_(0, step.weight_slots, step.weights[step.weight_rows])
+            step.weights = None
+        step.closed = True
 
     def _reserve(self, take):
         """Run a page reservation (all or nothing).  When the pool is exhausted while submitted
@@ -400,7 +504,7 @@ class PagedKVRunner:
     def synchronize(self) -> list[int]:
         """Wait for every submitted step's work, close all steps and release their pages."""
         for st in self._inflight:
-            st.closed = True
+            self._close(st)
             if st.event is not None:
                 st.event.synchronize()
         return self.reclaim()
