@@ -54,6 +54,8 @@ FILE_FLAGS = {
     # preloaded into scalar registers at dispatch, so its first loads (the step plan) do not wait
     # for the kernel-argument loads.
     "paged_decode_rows.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=9"],
+    # Likewise the 8-bit decode kernel's first ten (lengths, sizes, tables, query).
+    "paged_decode_fp8.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=10"],
 }
 
 

@@ -73,30 +73,44 @@ struct F8Workspace {
 };
 
 // Pages of row b in the list: its own, and kRowStart more in front when it has any.
+__device__ __forceinline__ int f8_row(const int32_t* seq_lens, const uint8_t* active, int b, int cap) {
+  const int sl = seq_lens[b];
+  const int act = active != nullptr ? int(active[b]) : 1;
+  const int n = ((act != 0 ? max(0, min(sl, cap)) : 0) + kF8Page - 1) / kF8Page;
+  return n > 0 ? n + kRowStart : 0;
+}
+__device__ __forceinline__ int f8_wave_scan(int x) {  // inclusive
+  const int lane = threadIdx.x % kWave;
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const int y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+// Offsets of the rows, s_cum[0 .. batch]; returns the total.  Up to 64 rows every wave computes (and stores) them all, so
+// that no wave waits for another.
 template <int kWaves>
 __device__ __forceinline__ int f8_offsets(int* s_cum, int* s_wsum, const int32_t* seq_lens, const uint8_t* active,
                                           int batch, int cap) {
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  if (batch <= kWave) {
+    const int n = lane < batch ? f8_row(seq_lens, active, lane, cap) : 0;
+    const int x = f8_wave_scan(n);
+    if (lane < batch) s_cum[lane] = x - n;
+    const int total = __builtin_amdgcn_readlane(x, kWave - 1);
+    if (lane == 0) s_cum[batch] = total;
+    return total;
+  }
   int running = 0;
   for (int base = 0; base < batch; base += kWaves * kWave) {
     const int i = base + tid;
-    int n = 0;
-    if (i < batch) {
-      const int sl = seq_lens[i];
-      const int act = active != nullptr ? int(active[i]) : 1;
-      const int len = act != 0 ? max(0, min(sl, cap)) : 0;
-      n = (len + kF8Page - 1) / kF8Page;
-      if (n > 0) n += kRowStart;
-    }
-    int x = n;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-      const int y = __shfl_up(x, o);
-      if (lane >= o) x += y;
-    }
+    const int n = i < batch ? f8_row(seq_lens, active, i, cap) : 0;
+    const int x = f8_wave_scan(n);
     if (lane == kWave - 1) s_wsum[wave] = x;
     __syncthreads();
     int pre = 0, tot = 0;
+#pragma unroll
     for (int w = 0; w < kWaves; ++w) {
       const int v = s_wsum[w];
       pre += w < wave ? v : 0;
@@ -153,10 +167,11 @@ __device__ __forceinline__ void f8_merge(__amdgpu_buffer_rsrc_t r_ml, __amdgpu_b
 
 template <int D, bool kAppend, bool kWeights>
 __global__ __launch_bounds__(kDecThreads, f8_per_simd(D)) void decode_fp8_kernel(
-    f16* __restrict__ out, const f16* __restrict__ q, F8Cache cache, const int32_t* __restrict__ block_tables,
-    int32_t max_pages, const int32_t* __restrict__ seq_lens, const uint8_t* __restrict__ active, int32_t batch,
-    int32_t hkv, int32_t G, int32_t max_len, float scale_log2, F8Workspace ws, F8Append ap,
-    float* __restrict__ page_weights, int32_t streams) {
+    const int32_t* __restrict__ seq_lens, const uint8_t* __restrict__ active, int32_t batch, int32_t max_pages,
+    int32_t max_len, int32_t hkv, int32_t G, int32_t streams, const int32_t* __restrict__ block_tables,
+    const f16* __restrict__ q,  // (up to here in registers at dispatch: build.py)
+    F8Cache cache, f16* __restrict__ out, float scale_log2, F8Workspace ws, F8Append ap,
+    float* __restrict__ page_weights) {
   constexpr int kKL = F8Page<D>::kKL, kVW = F8Page<D>::kVW;
   constexpr int kT = D / 16;   // output tiles (dims m D / 16 + tile)
   constexpr int kU = D / 16;   // 4-dim units of a lane's outputs: unit r (D / 64) + q = dims of row 4 g + r, 4 q ..
@@ -165,7 +180,7 @@ __global__ __launch_bounds__(kDecThreads, f8_per_simd(D)) void decode_fp8_kernel
   static_assert(kWave % S == 0, "windows are whole turns of the ring");
   constexpr int kEnt = 2 * kWaves;  // states a workgroup has at its end: at most two a wave
   __shared__ int s_wsum[kWaves];
-  __shared__ int s_row[kEnt], s_first[kEnt], s_last[kEnt];
+  __shared__ int s_row[kEnt], s_span[kEnt];  // a state's row (-1: none), and the workgroups that hold it: first << 16 | last
   __shared__ float s_m[kEnt][kF8MaxGroup], s_l[kEnt][kF8MaxGroup], s_tot[kF8MaxGroup];
   __shared__ uint32_t s_ticket[2];
   extern __shared__ __attribute__((aligned(16))) f32x4 s_o[];  // [kEnt][G D / 4], then the rows' offsets [batch + 1]
@@ -191,8 +206,14 @@ __global__ __launch_bounds__(kDecThreads, f8_per_simd(D)) void decode_fp8_kernel
   const int nr = min(min(streams, kMaxRanges * batch), (T + kMinPages - 1) / kMinPages);
   if (wg * kWaves >= nr) return;
   const bool works = stream < nr;  // (the workgroup's last waves may have no range)
-  const int t0 = works ? int(int64_t(T) * stream / nr) : T, t1 = works ? int(int64_t(T) * (stream + 1) / nr) : T;
-  auto range_of = [&](int t) -> int { return int((int64_t(t + 1) * nr - 1) / T); };
+  // the first `rem` ranges have base + 1 pages, the others base
+  const uint32_t base = uint32_t(T) / uint32_t(nr), rem = uint32_t(T) - base * nr, bend = rem * (base + 1);
+  const int t0 = works ? int(stream * base + min(uint32_t(stream), rem)) : T;
+  const int t1 = works ? t0 + int(base) + (uint32_t(stream) < rem ? 1 : 0) : T;
+  auto range_of = [&](int t) -> int {
+    const uint32_t u = uint32_t(t);
+    return int(u < bend ? u / (base + 1) : rem + (u - bend) / base);
+  };
 
   const int64_t v_codes = cache.num_pages * hkv * (kF8Page * D), v_scales = cache.num_pages * hkv;
   const uint32_t k_lane = n * D + 16 * g, v_lane = 4 * g * D + n * (D / 16);
@@ -533,8 +554,7 @@ __global__ __launch_bounds__(kDecThreads, f8_per_simd(D)) void decode_fp8_kernel
       }
       if (lane == 0) {
         s_row[en] = b;
-        s_first[en] = first;
-        s_last[en] = first + nranges - 1;
+        s_span[en] = (first / kWaves) << 16 | (first + nranges - 1) / kWaves;
       }
       ++npend;
     }
@@ -556,28 +576,37 @@ __global__ __launch_bounds__(kDecThreads, f8_per_simd(D)) void decode_fp8_kernel
     __syncthreads();
   };
   int open = 0, open_b[2] = {0, 0}, open_wg[2] = {0, 0}, open_np[2] = {0, 0};
-  for (int e0 = 0; e0 < kEnt;) {
-    const int b = s_row[e0];
-    if (b < 0) {
-      ++e0;
-      continue;
-    }
-    int e1 = e0 + 1;
-    while (e1 < kEnt && (s_row[e1] == b || s_row[e1] < 0)) ++e1;
-    const int wg0 = s_first[e0] / kWaves, wg1 = s_last[e0] / kWaves;
+  const int e_row = s_row[lane % kEnt], e_span = s_span[lane % kEnt];  // lane e: state e's
+  uint32_t todo = uint32_t(__builtin_amdgcn_ballot_w64(lane < kEnt && e_row >= 0));
+  while (todo != 0) {
+    const int e0 = __builtin_ctz(todo);
+    const int b = __builtin_amdgcn_readlane(e_row, e0), span = __builtin_amdgcn_readlane(e_span, e0);
+    const uint32_t of_row = uint32_t(__builtin_amdgcn_ballot_w64(lane < kEnt && e_row == b));
+    todo &= ~of_row;
+    const int wg0 = span >> 16, wg1 = span & 0xffff;
     const bool whole = wg0 == wg1;
     for (int u = tid; u < units; u += kWaves * kWave) {
       const int un = u % (4 * G) % G;
-      float M = kNegBig, L = 0.f;
-      f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-      for (int x = e0; x < e1; ++x)
-        if (s_row[x] == b) M = fmaxf(M, s_m[x][un]);
-      for (int x = e0; x < e1; ++x) {
-        if (s_row[x] != b) continue;
-        const float w = exp2_fast(s_m[x][un] - M);
-        const f32x4 v = s_o[x * units + u];
-        L = fmaf(w, s_l[x][un], L);
-        o = f32x4{fmaf(w, v[0], o[0]), fmaf(w, v[1], o[1]), fmaf(w, v[2], o[2]), fmaf(w, v[3], o[3])};
+      float em[kEnt], el[kEnt], M = kNegBig, L = 0.f;
+      f32x4 eo[kEnt], o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int x = 0; x < kEnt; ++x) {
+        if ((of_row >> x) & 1u) {
+          em[x] = s_m[x][un];
+          el[x] = s_l[x][un];
+          eo[x] = s_o[x * units + u];
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < kEnt; ++x)
+        if ((of_row >> x) & 1u) M = fmaxf(M, em[x]);
+#pragma unroll
+      for (int x = 0; x < kEnt; ++x) {
+        if ((of_row >> x) & 1u) {
+          const float w = exp2_fast(em[x] - M);
+          L = fmaf(w, el[x], L);
+          o = f32x4{fmaf(w, eo[x][0], o[0]), fmaf(w, eo[x][1], o[1]), fmaf(w, eo[x][2], o[2]), fmaf(w, eo[x][3], o[3])};
+        }
       }
       if (whole) {
         write_unit(b, u, o, L > 0.f ? 1.f / L : 0.f);
@@ -596,7 +625,6 @@ __global__ __launch_bounds__(kDecThreads, f8_per_simd(D)) void decode_fp8_kernel
       open_np[open & 1] = wg1 - wg0 + 1;
       ++open;
     }
-    e0 = e1;
   }
   if (open == 0) return;
   wait_all_mem();
@@ -690,8 +718,8 @@ static int f8_decode(void* out, const void* query, void* codes, float* scales, i
   const hipStream_t s = static_cast<hipStream_t>(stream);
   auto launch = [&](auto k) {
     k<<<dim3(unsigned(blocks)), dim3(kDecThreads), lds, s>>>(
-        static_cast<f16*>(out), static_cast<const f16*>(query), cache, block_tables, max_pages, seq_lens, active, batch,
-        hkv, G, cap, sl, ws, ap, page_weights, int32_t(streams));
+        seq_lens, active, batch, max_pages, cap, hkv, G, int32_t(streams), block_tables,
+        static_cast<const f16*>(query), cache, static_cast<f16*>(out), sl, ws, ap, page_weights);
   };
   auto pick = [&](auto dim) {
     constexpr int D = decltype(dim)::value;
