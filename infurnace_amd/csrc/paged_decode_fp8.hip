@@ -25,9 +25,10 @@
 //  * Page weights (kWeights): each page's log2-sum-exp per query head goes to the workspace; whoever finishes a
 //    (row, head) turns them into sum_g exp2(lse - total) and adds them to page_weights.
 //
-// What bounds it: memory, above about 100 MB.  128 rows of 1023-8190 keys, 32 / 8 heads x 128 (1.21 GB): 213 us, 5.7
-// TB/s; 32 rows of 128-4096, 16 / 8 heads (143 MB): 34 us, of which about 4 before a wave's first page (lengths, ids,
-// scales), 20 streaming, 3 of uneven waves and 7 after (states written through to memory, ticket, merge).
+// What bounds it: memory, above about 100 MB.  128 rows of 1023-8190 keys, 32 / 8 heads x 128 (1.21 GB): 203-213 us on
+// different cards, 5.7-6.0 TB/s; 32 rows of 128-4096, 16 / 8 heads (143 MB): 33 us, of which about 4 before a wave's
+// first page (lengths, ids, scales), 20 streaming, 3 of uneven waves and 6 after (states written through to memory,
+// ticket, merge).  One row of 512 keys: 8.6 us, all of it those steps.
 #include <algorithm>
 #include <type_traits>
 
@@ -36,22 +37,23 @@
 namespace ifn {
 
 // Threads of a workgroup.  Small ones: a workgroup's waves wait for each other before they merge (one row of 512
-// keys 10.2 us with 256, 12.6 with 512; 48 rows of 100-4000, 2 kv heads, 23.3 and 29.4).
+// keys 8.7 us with 256, 10.3 with 512; 48 rows of 100-4000, 2 kv heads, 22.5 and 24.2).
 constexpr int kDecThreads = 256;
 constexpr int kDecWaves = kDecThreads / kWave;
 constexpr int kDecPerSimd = 2;     // waves a SIMD is to hold (registers)
 constexpr int f8_per_simd(int d) { return d == 256 ? 1 : kDecPerSimd; }
-// Pages in a wave's ring.  The memory is as busy with 2 as with 4 (128 rows of 1023-8190 keys: 213 and 214 us), and
-// short pieces request fewer pages twice (32 rows of 128-4096: 35.2 and 37.1 us).
+// Pages in a wave's ring.  The memory is as busy with 2 as with 4 (128 rows of 1023-8190 keys: 203 and 204 us), and
+// short pieces request fewer pages twice (32 rows of 128-4096: 33.6 and 35.6 us).
 constexpr int kRing = 2;
 constexpr int kF8MaxBatch = 4096;  // rows per call (LDS offsets)
 constexpr int kF8MaxGroup = 16;    // query heads per kv head (MFMA columns)
 // Pages a row's start counts for in the split: its ids, scales and query take three round trips before the first
-// page (32 rows of 128-4096 keys: 37.1, 36.8 and 36.0 us with 1, 2 and 3; 64 rows of 256 dims 58.1, 56.3, 55.1).
-constexpr int kRowStart = 3;
+// page, and its state is merged.  With 3, 9 and 16: 48 rows of 100-4000 keys, 2 kv heads, 22.5, 20.3 and 20.2 us; 32
+// rows of 128-4096 33.5, 33.2 and 33.6; one row of 512 8.7, 8.6 and 9.2 (the start's own ranges have nothing to do).
+constexpr int kRowStart = 9;
 constexpr int kMinPages = 2;       // fewest list positions per range
 // Most ranges per row of the call.  A row's states are merged 16 workgroups a round trip, so more than 64 waves a row
-// cost another one (one row of 8000 keys, 32 / 8 heads: 17.9, 14.8, 15.6 and 20.4 us with 32, 64, 128 and 250 ranges).
+// cost another one (one row of 8000 keys, 32 / 8 heads: 16.2, 13.1, 14.2 and 18.8 us with 32, 64, 128 and 256 ranges).
 constexpr int kMaxRanges = 64;
 
 struct F8Cache {
@@ -651,12 +653,13 @@ __global__ __launch_bounds__(kDecThreads, f8_per_simd(D)) void decode_fp8_kernel
   }
 }
 
-// Streams of a call, whole workgroups of them: at most kWavesPerCu waves a CU over all kv heads, and no more than
-// the longest call of these sizes has ranges.
-constexpr int kWavesPerCu = 8;
-static int64_t f8_streams(int64_t batch, int32_t hkv, int32_t max_len, int cus) {
+// Streams of a call, whole workgroups of them: as many waves as the card holds at once, over all kv heads (64 rows of
+// 500-4000 keys x 256 dims, 2 kv heads: 37.8 us, 51.6 with twice as many), and no more than the longest call of these
+// sizes has ranges.
+constexpr int kSimdsPerCu = 4;
+static int64_t f8_streams(int64_t batch, int32_t hkv, int32_t d, int32_t max_len, int cus) {
   const int64_t most = ceil_div(ceil_div(batch * (ceil_div(max_len, kF8Page) + kRowStart), kMinPages), kDecWaves);
-  const int64_t wgs = int64_t(cus) * kWavesPerCu / kDecWaves / hkv;
+  const int64_t wgs = int64_t(cus) * kSimdsPerCu * f8_per_simd(d) / kDecWaves / hkv;
   return kDecWaves * std::max<int64_t>(1, std::min(most, wgs));
 }
 static size_t f8_ws_layout(int64_t batch, int64_t wgs, int32_t hkv, int32_t G, int32_t d, int32_t max_pages,
@@ -700,7 +703,7 @@ static int f8_decode(void* out, const void* query, void* codes, float* scales, i
   const int cus = device_cu_count();
   if (workspace == nullptr) return IFN_ERR_WORKSPACE;
   IFN_CHECK_ALIGN16(workspace);
-  const int64_t streams = f8_streams(batch, hkv, cap, std::max(1, cus));
+  const int64_t streams = f8_streams(batch, hkv, d, cap, std::max(1, cus));
   size_t off_ml, off_o, off_lse;
   if (workspace_bytes < f8_ws_layout(batch, streams / kDecWaves, hkv, G, d, max_pages, page_weights != nullptr, &off_ml, &off_o,
                                      &off_lse))
@@ -744,7 +747,7 @@ extern "C" size_t ifn_paged_decode_fp8_workspace_bytes(int32_t batch, int32_t nu
       block_size < 1 || max_pages_per_seq < 1 || max_seq_len < 0)
     return 0;
   const int64_t cap = std::min<int64_t>(int64_t(max_pages_per_seq) * kF8Page, max_seq_len);
-  const int64_t wgs = f8_streams(batch, num_kv_heads, int32_t(cap), std::max(1, device_cu_count())) / kDecWaves;
+  const int64_t wgs = f8_streams(batch, num_kv_heads, head_dim, int32_t(cap), std::max(1, device_cu_count())) / kDecWaves;
   size_t a, b, c;
   return f8_ws_layout(batch, wgs, num_kv_heads, num_q_heads / num_kv_heads, head_dim, max_pages_per_seq,
                       page_weights != 0, &a, &b, &c);
