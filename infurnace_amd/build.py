@@ -54,8 +54,11 @@ FILE_FLAGS = {
     # preloaded into scalar registers at dispatch, so its first loads (the step plan) do not wait
     # for the kernel-argument loads.
     "paged_decode_rows.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=9"],
-    # Likewise the 8-bit decode kernel's first ten (lengths, sizes, tables, query).
+    # Likewise what the first loads of the 8-bit and eviction kernels need (lengths or slots, sizes, tables).
     "paged_decode_fp8.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=10"],
+    "paged_prefill_fp8.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=9"],
+    "kv_store_fp8.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=6"],
+    "evict_pages.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=9"],
 }
 
 

@@ -14,8 +14,8 @@
 // order.
 //
 // What bounds it: latency -- lengths, sums, up to three passes, the scan, the row, one after the other.  32 rows of 8-256
-// pages, 8 heads: 7.5 us (ranking by counting instead of the passes: 8.8-9.8); 64 rows of 1250-4096 pages (17 MB read and
-// written): 13.5 us, where one workgroup a row that also wrote the zeros took 24.
+// pages, 8 heads: 6.7 us (ranking by counting instead of the passes: 1.3-2.3 more); 64 rows of 1250-4096 pages (17 MB
+// read and written): 12.8 us, where one workgroup a row that also wrote the zeros took 24.
 #include <algorithm>
 
 #include "ifn_common.hpp"
@@ -60,10 +60,11 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* s_sum, uint
 }
 
 __global__ __launch_bounds__(kEvictThreads) void evict_pages_kernel(
-    int32_t* __restrict__ out_tables, int32_t* __restrict__ out_lens, float* __restrict__ out_weights,
-    int32_t* __restrict__ num_evicted, const int32_t* __restrict__ tables, int32_t max_pages,
     const int32_t* __restrict__ lens, const uint8_t* __restrict__ active, const float* __restrict__ weights,
-    int32_t hkv, int32_t keep, int32_t sink, int32_t recent) {
+    int32_t max_pages, int32_t hkv, int32_t keep, int32_t sink, int32_t recent,
+    const int32_t* __restrict__ tables,  // (up to here in registers at dispatch: build.py)
+    int32_t* __restrict__ out_tables, int32_t* __restrict__ out_lens, float* __restrict__ out_weights,
+    int32_t* __restrict__ num_evicted) {
   extern __shared__ uint32_t s_key[];  // max_pages: the keys, then the row's permutation
   __shared__ int s_hist[kEvictBins];
   __shared__ uint32_t s_sum[kEvictWaves];
@@ -201,9 +202,9 @@ extern "C" int ifn_evict_pages(int32_t* out_tables, int32_t* out_lens, float* ou
       int64_t(std::min(keep_pages, max_pages_per_seq)) * num_kv_heads >= int64_t(1) << 31)
     return IFN_ERR_UNSUPPORTED;
   if (batch == 0) return IFN_OK;
-  evict_pages_kernel<<<dim3(unsigned(batch), unsigned(1 + std::min<int32_t>(num_kv_heads, 32))), dim3(kEvictThreads), size_t(max_pages_per_seq) * 4,
-                       static_cast<hipStream_t>(stream)>>>(
-      out_tables, out_lens, out_weights, num_evicted, block_tables, max_pages_per_seq, seq_lens, active_mask,
-      page_weights, num_kv_heads, keep_pages, sink_pages, recent_pages);
+  evict_pages_kernel<<<dim3(unsigned(batch), unsigned(1 + std::min<int32_t>(num_kv_heads, 32))), dim3(kEvictThreads),
+                       size_t(max_pages_per_seq) * 4, static_cast<hipStream_t>(stream)>>>(
+      seq_lens, active_mask, page_weights, max_pages_per_seq, num_kv_heads, keep_pages, sink_pages, recent_pages,
+      block_tables, out_tables, out_lens, out_weights, num_evicted);
   return ifn_launch_status();
 }

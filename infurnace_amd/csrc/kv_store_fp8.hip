@@ -14,8 +14,8 @@
 // is stored).  D / 8 lanes take a row, 8 dims each: a load instruction reads whole rows of a head, a store writes
 // whole lines of a block.
 //
-// What bounds it: small calls by their round trips (slots, rows and scales, stores), 4.4 us; large ones by memory (8192
-// tokens of 8 x 128: 12.0 us, 4.2 TB/s; 30000: 34.6 us, 5.3 TB/s, where a large copy reaches 4.7).
+// What bounds it: small calls by their round trips (slots, rows and scales, stores), 3.9 us; large ones by memory (8192
+// tokens of 8 x 128: 11.8 us, 4.3 TB/s; 30000: 34.6 us, 5.3 TB/s, where a large copy reaches 4.7).
 #include "kv_fp8.hpp"
 
 namespace ifn {
@@ -35,9 +35,10 @@ __device__ __forceinline__ float wave_max_fast(float x) {
 // per: consecutive tokens a wave looks at for first ones.
 template <int D>
 __global__ __launch_bounds__(kStoreF8Threads) void store_kv_fp8_kernel(
-    uint8_t* __restrict__ codes, float* __restrict__ scales, int64_t num_pages, const int32_t* __restrict__ slots,
-    const uint8_t* __restrict__ active, const f16* __restrict__ new_k, const f16* __restrict__ new_v,
-    int32_t num_tokens, int32_t hkv, int32_t per) {
+    const int32_t* __restrict__ slots, const uint8_t* __restrict__ active, int64_t num_pages, int32_t num_tokens,
+    int32_t hkv, int32_t per,  // (up to here in registers at dispatch: build.py)
+    uint8_t* __restrict__ codes, float* __restrict__ scales, const f16* __restrict__ new_k,
+    const f16* __restrict__ new_v) {
   constexpr int kLanes = D / 8;           // lanes per row
   constexpr int kRows = kWave / kLanes;   // rows per instruction
   constexpr int kC = kF8Page / kRows;     // instructions per block: instruction c, rows kRows c + lane / kLanes
@@ -155,7 +156,7 @@ extern "C" int ifn_store_kv_fp8(void* codes_layer, float* scales_layer, int64_t 
   const hipStream_t s = static_cast<hipStream_t>(stream);
   auto k = head_dim == 64 ? store_kv_fp8_kernel<64> : head_dim == 128 ? store_kv_fp8_kernel<128> : store_kv_fp8_kernel<256>;
   k<<<dim3(unsigned(blocks)), dim3(kStoreF8Threads), 0, s>>>(
-      static_cast<uint8_t*>(codes_layer), scales_layer, num_pages, slot_mapping, active_mask,
-      static_cast<const f16*>(new_k), static_cast<const f16*>(new_v), num_tokens, num_kv_heads, per);
+      slot_mapping, active_mask, num_pages, num_tokens, num_kv_heads, per, static_cast<uint8_t*>(codes_layer),
+      scales_layer, static_cast<const f16*>(new_k), static_cast<const f16*>(new_v));
   return ifn_launch_status();
 }

@@ -14,7 +14,7 @@
 // tile again, so calls that fill the chip in workgroups of 128 columns go to paged_prefill_fp8_block.hip.
 //
 // What bounds it: vector work and the L2 (8 KB a tile of 32 x 32), about 0.9 us a tile and SIMD whether it has one
-// wave or two.  512 queries at 1024, 16 / 8 heads x 128 (5.4 GFLOP): 16.6 us, of which 3 before the first tile and 3.5
+// wave or two.  512 queries at 1024, 16 / 8 heads x 128 (5.4 GFLOP): 15.7 us, of which 3 before the first tile and 3.5
 // to merge; 16 queries at 4096: 13.3 us.
 #include <algorithm>
 
@@ -30,9 +30,10 @@ constexpr int kPfCols = 16 * kPfTiles;
 
 template <int D>
 __global__ __launch_bounds__(kPfThreads, 2) void prefill_fp8_kernel(
-    f16* __restrict__ out, const f16* __restrict__ q, const uint8_t* __restrict__ codes,
-    const float* __restrict__ scales, int64_t num_pages, const int32_t* __restrict__ table, int32_t query_start,
-    int32_t T, int32_t hkv, int32_t G, int32_t n_blocks, float scale_log2, int32_t nsplit, PrefillWorkspace ws) {
+    const int32_t* __restrict__ table, const f16* __restrict__ q, int64_t num_pages, int32_t query_start, int32_t T,
+    int32_t hkv, int32_t G, int32_t n_blocks, int32_t nsplit,  // (up to here in registers at dispatch: build.py)
+    const float* __restrict__ scales, const uint8_t* __restrict__ codes, f16* __restrict__ out, float scale_log2,
+    PrefillWorkspace ws) {
   constexpr int kKL = F8Page<D>::kKL, kVW = F8Page<D>::kVW;
   constexpr int kT = D / 16, NC = kPfTiles, KW = kPfWaves;
   __shared__ f32x4 s_o[KW][NC * kT][kWave];
@@ -441,7 +442,7 @@ extern "C" int ifn_paged_prefill_fp8(void* out, const void* query, const void* c
                             reinterpret_cast<float*>(w + off_o)};
   auto k = head_dim == 64 ? prefill_fp8_kernel<64> : prefill_fp8_kernel<128>;
   k<<<dim3(unsigned(n_blocks * num_kv_heads * plan.nsplit)), dim3(kPfThreads), 0, s>>>(
-      o, q, codes, scales_layer, num_pages, block_table, query_start, num_q_tokens, num_kv_heads, G, int32_t(n_blocks), sl,
-      plan.nsplit, ws);
+      block_table, q, num_pages, query_start, num_q_tokens, num_kv_heads, G, int32_t(n_blocks), plan.nsplit,
+      scales_layer, codes, o, sl, ws);
   return ifn_launch_status();
 }
