@@ -56,7 +56,7 @@ FILE_FLAGS = {
     "paged_decode_rows.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=9"],
     # Likewise what the first loads of the 8-bit and eviction kernels need (lengths or slots, sizes, tables).
     "paged_decode_fp8.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=10"],
-    "paged_prefill_fp8.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=9"],
+    "paged_prefill_fp8.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=9", "-fno-honor-nans"],
     "kv_store_fp8.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=6"],
     "evict_pages.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=9"],
 }

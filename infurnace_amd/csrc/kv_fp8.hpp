@@ -152,6 +152,12 @@ __device__ __forceinline__ f16x8 f8_frag(uint32_t w0, uint32_t w1, float s0, flo
   return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// A score, or -inf where it is not kept: by its bits, since the score of a row that nobody stored may be NaN, which
+// the prefill files' float operations are compiled not to expect.
+__device__ __forceinline__ float f8_masked(bool keep, float s) {
+  return __builtin_bit_cast(float, keep ? __builtin_bit_cast(uint32_t, s) : 0xff800000u);
+}
+
 // No instruction: the values must have arrived at this point.
 template <class A, class B>
 __device__ __forceinline__ void settle(A& a, B& b) {

@@ -43,9 +43,9 @@ __global__ __launch_bounds__(kStoreF8Threads) void store_kv_fp8_kernel(
   constexpr int kRows = kWave / kLanes;   // rows per instruction
   constexpr int kC = kF8Page / kRows;     // instructions per block: instruction c, rows kRows c + lane / kLanes
   const int lane = threadIdx.x % kWave;
-  const int64_t w = int64_t(blockIdx.x) * kStoreF8Waves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int h = int(w % hkv);
-  const int64_t t0 = w / hkv * per;
+  const uint32_t w = blockIdx.x * kStoreF8Waves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int h = int(w % uint32_t(hkv));
+  const int64_t t0 = int64_t(w / uint32_t(hkv)) * per;
   if (t0 >= num_tokens) return;
   const int64_t num_slots = num_pages * kF8Page;
   // slots of the 64 tokens before t0, from t0 on, and after those; -1 where nothing is stored
@@ -152,7 +152,7 @@ extern "C" int ifn_store_kv_fp8(void* codes_layer, float* scales_layer, int64_t 
   const int32_t per = most <= 2048 ? 1 : most <= 8192 ? 4 : kF8Page;
   const int64_t waves = ceil_div(num_tokens, per) * num_kv_heads;
   const int64_t blocks = ceil_div(waves, kStoreF8Waves);
-  if (blocks >= int64_t(1) << 31) return IFN_ERR_UNSUPPORTED;
+  if (waves >= int64_t(1) << 31) return IFN_ERR_UNSUPPORTED;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   auto k = head_dim == 64 ? store_kv_fp8_kernel<64> : head_dim == 128 ? store_kv_fp8_kernel<128> : store_kv_fp8_kernel<256>;
   k<<<dim3(unsigned(blocks)), dim3(kStoreF8Threads), 0, s>>>(

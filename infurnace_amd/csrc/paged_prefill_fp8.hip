@@ -46,9 +46,9 @@ __global__ __launch_bounds__(kPfThreads, 2) void prefill_fp8_kernel(
   const int h = int(blockIdx.x) % hkv, rest = int(blockIdx.x) / hkv;
   const int split = rest % nsplit, blk = n_blocks - 1 - rest / nsplit;
   const int hq = hkv * G;
-  const int64_t c0 = int64_t(blk) * kPfCols, cols = int64_t(T) * G;
-  const int keys = query_start + int(min(c0 + kPfCols - 1, cols - 1) / G) + 1;  // keys some column sees
-  const int first_pos = query_start + int(c0 / G);        // every column sees keys up to this one
+  const uint32_t c0 = uint32_t(blk) * kPfCols, cols = uint32_t(T) * G;  // (the host: rows below 2^31)
+  const int keys = query_start + int(min(c0 + kPfCols - 1, cols - 1) / uint32_t(G)) + 1;  // keys some column sees
+  const int first_pos = query_start + int(c0 / uint32_t(G));        // every column sees keys up to this one
   const int pages = (keys + kF8Page - 1) / kF8Page, tiles = (pages + 1) / 2;
   const int stride = KW * nsplit, lead = KW * split + wave;
   const int mine = (tiles - lead + stride - 1) / stride, last = mine - 1;  // this wave's tiles: lead + stride i
@@ -64,14 +64,14 @@ __global__ __launch_bounds__(kPfThreads, 2) void prefill_fp8_kernel(
   int win = 0, ids = load_ids(0), ids1 = load_ids(1);
 
   int my_pos[NC];
-  int64_t my_row[NC];  // (query, head) row of the lane's column of each tile
+  uint32_t my_row[NC];  // (query, head) row of the lane's column of each tile
   f16x8 qf[NC][2 * kKL];
 #pragma unroll
   for (int x = 0; x < NC; ++x) {
-    const int64_t c = min(c0 + 16 * x + n, cols - 1);
-    my_pos[x] = query_start + int(c / G);
-    my_row[x] = (c / G) * hq + h * G + c % G;
-    const f16* qp = q + my_row[x] * D + 16 * g;
+    const uint32_t c = min(c0 + 16 * x + n, cols - 1), t = c / uint32_t(G);
+    my_pos[x] = query_start + int(t);
+    my_row[x] = t * hq + h * G + (c - t * G);
+    const f16* qp = q + int64_t(my_row[x]) * D + 16 * g;
 #pragma unroll
     for (int i = 0; i < kKL; ++i) {
       qf[x][2 * i] = as_h8(ld16(qp + 64 * i));
@@ -125,7 +125,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void prefill_fp8_kernel(
         for (int x = 0; x < NC; ++x) {
           const int lim = live[y] ? my_pos[x] - key0 - 16 * y - 4 * g : -1;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[x][y][j] = j <= lim ? s[x][y][j] : -INFINITY;
+          for (int j = 0; j < 4; ++j) s[x][y][j] = f8_masked(j <= lim, s[x][y][j]);
         }
         const int end = live[y] ? keys - key0 - 16 * y - 4 * g : 0;  // (rows nobody stored may hold NaN, and 0 x NaN is NaN)
 #pragma unroll
@@ -412,7 +412,8 @@ extern "C" int ifn_paged_prefill_fp8(void* out, const void* query, const void* c
     return IFN_ERR_INVALID_ARGUMENT;
   if (block_size != kF8Page || (head_dim != 64 && head_dim != 128)) return IFN_ERR_UNSUPPORTED;
   if (int64_t(query_start) + num_q_tokens > int64_t(max_pages) * kF8Page) return IFN_ERR_INVALID_ARGUMENT;
-  if (int64_t(query_start) + num_q_tokens > (int64_t(1) << 31) - 64 || num_pages > (int64_t(1) << 31) / kF8Page)
+  if (int64_t(query_start) + num_q_tokens > (int64_t(1) << 31) - 64 || num_pages > (int64_t(1) << 31) / kF8Page ||
+      int64_t(num_q_tokens) * num_q_heads > (int64_t(1) << 31) - 256)
     return IFN_ERR_UNSUPPORTED;
   IFN_CHECK_ALIGN16(out);
   IFN_CHECK_ALIGN16(query);

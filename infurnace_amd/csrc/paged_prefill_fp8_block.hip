@@ -79,15 +79,14 @@ __global__ __launch_bounds__(KS * kP8Threads, 2) void prefill_fp8_block_kernel(
   const int wave = wv % kP8Waves, grp = wv / kP8Waves;
   const int col = lane % 32, half = lane / 32;
   const int hq = hkv * G;
-  const int64_t cols = int64_t(T) * G, c0 = int64_t(blk) * kP8Cols;
-  const int64_t wc0 = c0 + 32 * wave;
-  const int64_t my_c = min(wc0 + col, cols - 1);
-  const int my_q = int(my_c / G), my_h = h * G + int(my_c % G);
+  const uint32_t cols = uint32_t(T) * G, c0 = uint32_t(blk) * kP8Cols, wc0 = c0 + 32 * wave;  // (the host: below 2^31)
+  const uint32_t my_c = min(wc0 + col, cols - 1), per_q = uint32_t(G);
+  const int my_q = int(my_c / per_q), my_h = h * G + int(my_c % per_q);
   const int my_pos = query_start + my_q;
   const int total = query_start + T;
-  const int n_tiles = int(ceil_div(query_start + int(min(c0 + kP8Cols - 1, cols - 1) / G) + 1, kP8Tile));
-  const int wave_first = query_start + int(min(wc0, cols - 1) / G);
-  const int wave_tiles = int(ceil_div(query_start + int(min(wc0 + 31, cols - 1) / G) + 1, kP8Tile));
+  const int n_tiles = int(ceil_div(query_start + int(min(c0 + kP8Cols - 1, cols - 1) / per_q) + 1, kP8Tile));
+  const int wave_first = query_start + int(min(wc0, cols - 1) / per_q);
+  const int wave_tiles = int(ceil_div(query_start + int(min(wc0 + 31, cols - 1) / per_q) + 1, kP8Tile));
 
   // Page ids and scales, 64 pages per window (16 tiles), one per lane, a window ahead.
   const int seq_pages = int(ceil_div(total, kF8Page));
@@ -209,7 +208,7 @@ __global__ __launch_bounds__(KS * kP8Threads, 2) void prefill_fp8_block_kernel(
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int lp = ((ti.fl >> (2 * j + r / 8)) & 1) ? lim - 4 * half : -1;
-          st[j][r] = 32 * j + 8 * (r / 4) + r % 4 <= lp ? st[j][r] : -INFINITY;
+          st[j][r] = f8_masked(32 * j + 8 * (r / 4) + r % 4 <= lp, st[j][r]);
         }
     }
   };

@@ -307,6 +307,28 @@ def test_prefill_large(dev, hq, hkv, d, t, start):
     check(paged_attention_fp8(q.to(dev), kv, sc, i32(table, dev), None, query_start=start), out, tol)
 
 
+@pytest.mark.parametrize("hq,hkv,d,t,start", [(32, 8, 128, 1101, 0), (32, 8, 128, 600, 1500), (16, 8, 128, 2103, 2),
+                                              (32, 8, 64, 1101, 3400), (36, 2, 128, 1901, 6)])
+def test_prefill_blocks(dev, hq, hkv, d, t, start):
+    """Calls that fill the chip, one and two key groups: NaN behind the sequence's end, a page outside the pool."""
+    say(f"prefill fp8 blocks hq={hq} hkv={hkv} d={d} t={t} start={start}")
+    rng = np.random.default_rng(t)
+    gen = torch.Generator().manual_seed(t + start)
+    total = start + t
+    table, pages = tables(rng, [total])
+    ref = random_cache(pages, hkv, d, start)
+    kv, sc = ref.to(dev)
+    assert total % 16
+    kv.view(torch.uint8)[:, int(table[0, total // 16]), :, total % 16:] = 0x7f
+    bad = table[0].copy()
+    bad[total // 32] = -5
+    live = torch.tensor([j // 16 != total // 32 for j in range(total)])
+    q = torch.randn((t, hq, d), generator=gen).half()
+    k, v = gather(ref.values(), table[0], total)
+    out, tol, _, _ = attend(q, k[live], v[live], torch.cumsum(live.long(), 0)[start:])
+    check(paged_attention_fp8(q.to(dev), kv, sc, i32(bad, dev), None, query_start=start), out, tol)
+
+
 def test_prefill_strange_pages(dev):
     say("prefill fp8 strange pages")
     rng = np.random.default_rng(2)
