@@ -519,10 +519,10 @@ int ifn_copy_pages(void* kv_pool, int32_t num_layers, int64_t num_pages, const i
  * them has offset 0 in the page the block starts anew (scale = need, its rows
  * that are not stored become zero), else its scale becomes max(scale, need) and
  * its other codes are rounded to a grown scale.  A page is filled from offset 0
- * up, so rows behind the stored ones are zero.  The tokens of one page must lie
- * within 64 consecutive entries of slot_mapping (any order; of two active entries
- * with one slot the later is stored): a token farther than that from the first of
- * its page may be dropped or race with it.
+ * up, so rows behind the stored ones are zero.  The call's tokens may be in any
+ * order (a sequence's side by side and in order are the fastest).  Active slots
+ * are distinct: of two equal ones at most 64 entries apart the later is stored,
+ * farther apart the block may mix both rows.
  * Replaces: store_kv, docs/architecture.md:245 (placeholder
  * src/infurnace/kernels/kv_store.py, 0 B), for a cache of half the bytes; the
  * reference stores fp16 only.

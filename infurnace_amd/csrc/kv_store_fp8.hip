@@ -9,10 +9,11 @@
 //   c'[o_t] = e4m3(x_t / s')
 //
 // A block is changed as a whole, so one wave owns a page's two blocks of a head: the wave of the call's first token in
-// that page (a token has none of its page among the 63 before it), which finds the page's other tokens among the 63
-// that follow.  A call keeps a page's tokens that near to each other (any order; of two with one slot the later
-// is stored).  D / 8 lanes take a row, 8 dims each: a load instruction reads whole rows of a head, a store writes
-// whole lines of a block.
+// that page.  It looks at the 63 tokens before its own and after it.  That is enough where the page's tokens are
+// a run in order that starts at offset 0 or with the call and ends at offset 15 or with it (a chunk's are; slots are
+// distinct), or where the call has no more tokens; otherwise it goes through all slots of the call.  Of two tokens
+// with one slot the later is stored.  D / 8 lanes take a row, 8 dims each: a load instruction reads whole rows of a
+// head, a store writes whole lines of a block.
 //
 // What bounds it: small calls by their round trips (slots, rows and scales, stores), 3.9 us; large ones by memory (8192
 // tokens of 8 x 128: 11.8 us, 4.3 TB/s; 30000: 34.6 us, 5.3 TB/s, where a large copy reaches 4.7).
@@ -75,12 +76,36 @@ __global__ __launch_bounds__(kStoreF8Threads) void store_kv_fp8_kernel(
     // the block's rows in this call, as tokens from t0: a run of the page's tokens in order, or the latest of each offset
     int from[kC];
     const uint64_t b1 = __builtin_amdgcn_ballot_w64(m1), b2 = __builtin_amdgcn_ballot_w64(m2);
-    if (b2 == 0 && __builtin_amdgcn_ballot_w64(m1 && s1 - slot != lane - i) == 0) {
-      const int end = (slot & 15) + __builtin_popcountll(b1);
+    const uint64_t r1 = b1 >> i;
+    const bool run = b2 == 0 && (r1 & (r1 + 1)) == 0 && __builtin_amdgcn_ballot_w64(m1 && s1 - slot != lane - i) == 0;
+    const int off = slot & 15, end = off + __builtin_popcountll(b1);
+    const bool whole = run && (off == 0 || t0 + i == 0) && (end == kF8Page || t0 + i + end - off == num_tokens);
+    if (!whole && (t0 + i >= kWave || t0 + i + kWave < num_tokens)) {
+#pragma unroll
+      for (int c = 0; c < kC; ++c) from[c] = -1;
+      bool first = true;
+      for (int64_t at = 0; at < num_tokens && first; at += 4 * kWave) {
+        int s[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s[x] = slot_at(at + kWave * x + lane);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          for (uint64_t of = __builtin_amdgcn_ballot_w64((s[x] >> 4) == page); of != 0; of &= of - 1) {
+            const int j = __builtin_ctzll(of), o = __builtin_amdgcn_readlane(s[x], j) & 15;
+            const int f = int(at + kWave * x + j - t0);
+            first = first && f >= i;
+#pragma unroll
+            for (int c = 0; c < kC; ++c)
+              if (kRows * c + row0 == o) from[c] = f;
+          }
+        }
+      }
+      if (!first) continue;
+    } else if (run) {
 #pragma unroll
       for (int c = 0; c < kC; ++c) {
         const int row = kRows * c + row0;
-        from[c] = row >= (slot & 15) && row < end ? i + row - (slot & 15) : -1;
+        from[c] = row >= off && row < end ? i + row - off : -1;
       }
     } else {
 #pragma unroll

@@ -94,25 +94,16 @@ def _check_rows(name: str, t, shape: tuple, device, err: type[ValueError]) -> No
 
 
 def _validate_slots(slots: torch.Tensor, active, num_slots: int) -> None:
-    """Validate mode: active slots in the pool and distinct, a page's tokens within 64 consecutive entries."""
+    """Validate mode: active slots in the pool and distinct."""
     s = slots.detach().cpu().long()
-    at = torch.arange(s.numel())
     if active is not None:
-        on = active.detach().cpu().bool()
-        s, at = s[on], at[on]
+        s = s[active.detach().cpu().bool()]
     if s.numel() == 0:
         return
     if int(s.min()) < 0 or int(s.max()) >= num_slots:
         raise KVStoreError(f"active slot outside [0, {num_slots})")
     if s.numel() != torch.unique(s).numel():
         raise KVStoreError("two active rows map to the same slot")
-    page = s // BLOCK
-    _, where = torch.unique(page, return_inverse=True)
-    n = int(where.max()) + 1
-    first = torch.full((n,), 1 << 40).scatter_reduce_(0, where, at, "amin")
-    last = torch.zeros(n, dtype=torch.long).scatter_reduce_(0, where, at, "amax")
-    if bool((last - first > 63).any()):
-        raise KVStoreError("the tokens of one page are more than 63 entries apart in slot_mapping")
 
 
 def _validate_scales(scales: torch.Tensor, table: torch.Tensor, keys: torch.Tensor) -> None:
@@ -131,9 +122,9 @@ def store_kv_fp8(kv_pool: torch.Tensor, scales: torch.Tensor, slot_mapping: torc
 
     ``slot_mapping`` int32 [T] and ``active_mask`` bool/uint8 [T] or None as for ``store_kv``: rows that are
     inactive or whose slot is outside the pool write nothing.  A page is filled from its offset 0 up: the
-    token at offset 0 starts its blocks anew.  The tokens of one page lie within 64 consecutive entries
-    (every chunk and every step does); of two rows with one slot the later is stored.  ``validate=True``
-    adds a synchronising host check of the slots.
+    token at offset 0 starts its blocks anew.  A call's tokens may be in any order, those of a sequence in
+    order side by side being the fastest.  Active slots are distinct; ``validate=True`` adds a
+    synchronising host check of that.
     """
     if not validate and _fast.store_fp8(kv_pool, scales, slot_mapping, active_mask, new_k, new_v, layer) is not None:
         return None

@@ -75,6 +75,62 @@ def test_append_masks_order_and_strangers(dev, n):
     ref.same(kv, sc)
 
 
+@pytest.mark.parametrize("hkv,d", [(2, 64), (8, 128), (1, 256)])
+@pytest.mark.parametrize("n,start", [(30, 0), (300, 5), (1000, 0), (3001, 11)])
+def test_append_masked_chunk(dev, hkv, d, n, start):
+    """A chunk in order with rows masked out of its middle."""
+    say(f"append masked chunk hkv={hkv} d={d} n={n} start={start}")
+    rng = np.random.default_rng(n)
+    gen = torch.Generator().manual_seed(n + d)
+    pages = (start + n + 15) // 16
+    ref = random_cache(pages, hkv, d, n)
+    kv, sc = ref.to(dev)
+    slots = np.arange(start, start + n)
+    active = rng.random(n) < 0.9
+    k, v = rows(gen, n, hkv, d), rows(gen, n, hkv, d, 20.0)
+    store_kv_fp8(kv, sc, i32(slots, dev), torch.as_tensor(active).to(dev), k.to(dev), v.to(dev), validate=True)
+    ref.store(slots.tolist(), k, v, active)
+    ref.same(kv, sc)
+
+
+@pytest.mark.parametrize("hkv,d,seqs,each,start", [(2, 64, 65, 2, 3), (2, 128, 100, 16, 0), (1, 256, 70, 5, 12),
+                                                   (8, 128, 300, 20, 0), (8, 64, 513, 3, 14)])
+def test_append_position_major(dev, hkv, d, seqs, each, start):
+    """A step of several tokens a sequence, every sequence's first, then every sequence's second: a page's tokens are
+    `seqs` entries apart."""
+    say(f"append position major hkv={hkv} d={d} seqs={seqs} each={each}")
+    rng = np.random.default_rng(seqs)
+    gen = torch.Generator().manual_seed(seqs)
+    per = (start + each + 15) // 16
+    ids = rng.permutation(seqs * per).reshape(seqs, per)
+    ref = random_cache(seqs * per, hkv, d, seqs)
+    kv, sc = ref.to(dev)
+    pos = np.arange(start, start + each)
+    slots = (ids[:, pos // 16] * 16 + pos % 16).T.reshape(-1)
+    n = seqs * each
+    k, v = rows(gen, n, hkv, d), rows(gen, n, hkv, d, 20.0)
+    store_kv_fp8(kv, sc, i32(slots, dev), None, k.to(dev), v.to(dev), validate=True)
+    ref.store(slots.tolist(), k, v)
+    ref.same(kv, sc)
+
+
+@pytest.mark.parametrize("n", [200, 2500])
+def test_append_any_order(dev, n):
+    """Slots of a few pages in a random order over the whole call, inactive rows among them."""
+    say(f"append any order n={n}")
+    rng = np.random.default_rng(n)
+    gen = torch.Generator().manual_seed(n)
+    pages = 200
+    ref = random_cache(pages, 4, 128, n)
+    kv, sc = ref.to(dev)
+    slots = rng.permutation(pages * 16)[:n]
+    active = rng.random(n) < 0.7
+    k, v = rows(gen, n, 4, 128, 20.0), rows(gen, n, 4, 128)
+    store_kv_fp8(kv, sc, i32(slots, dev), torch.as_tensor(active).to(dev), k.to(dev), v.to(dev), validate=True)
+    ref.store(slots.tolist(), k, v, active)
+    ref.same(kv, sc)
+
+
 def test_append_extremes(dev):
     """fp16's smallest and largest numbers, zeros, and the borders of a scale (448, and the next number)."""
     say("append extremes")

@@ -137,7 +137,4 @@ def test_validate_slots():
         _validate_slots(s([0, 64]), None, 64)
     with pytest.raises(KVStoreError, match="same slot"):
         _validate_slots(s([3, 5, 3]), None, 64)
-    near, far = [0] + list(range(16, 78)) + [1], [0] + list(range(16, 79)) + [1]
-    _validate_slots(s(near), None, 256)
-    with pytest.raises(KVStoreError, match="63 entries"):
-        _validate_slots(s(far), None, 256)
+    _validate_slots(s([0] + list(range(16, 200)) + [1]), None, 256)  # (a page's tokens may be any distance apart)
