@@ -15,8 +15,8 @@
 // with one slot the later is stored.  D / 8 lanes take a row, 8 dims each: a load instruction reads whole rows of a
 // head, a store writes whole lines of a block.
 //
-// What bounds it: small calls by their round trips (slots, rows and scales, stores), 3.9 us; large ones by memory (8192
-// tokens of 8 x 128: 11.8 us, 4.3 TB/s; 30000: 34.6 us, 5.3 TB/s, where a large copy reaches 4.7).
+// What bounds it: small calls by their round trips (slots, rows and scales, stores), 4.1 us; large ones by memory (8192
+// tokens of 8 x 128: 11.9 us, 4.2 TB/s; 30000: 34.6 us, 5.3 TB/s, where a large copy reaches 4.7).
 #include "kv_fp8.hpp"
 
 namespace ifn {
@@ -170,9 +170,9 @@ extern "C" int ifn_store_kv_fp8(void* codes_layer, float* scales_layer, int64_t 
   IFN_CHECK_ALIGN16(new_k);
   IFN_CHECK_ALIGN16(new_v);
   if (num_tokens == 0) return IFN_OK;
-  // A wave for every token is best for the tokens of a step, each in a page of its own (8 heads, 256 of them: 5.1 us,
-  // 10.2 with four a wave, 32 with 16), a wave for every 16 for a chunk (2000 tokens: 22.4, 10.5, 5.5).  By what the
-  // call most likely is: steps have few tokens.  (512 tokens: a chunk 7.2, 5.3, 5.1, a step 6.9, 10.7, 32.9.)
+  // A wave for every token is best for the tokens of a step, each in a page of its own (8 heads, 256 of them: 5.8 us,
+  // 12.9 with four a wave, 43 with 16), a wave for every 16 for a chunk (2000 tokens: 22.2, 10.5, 5.5).  By what the
+  // call most likely is: steps have few tokens.  (512 tokens: a chunk 7.2, 5.2, 4.9, a step 8.1, 15.7, 55.)
   const int64_t most = int64_t(num_tokens) * num_kv_heads;
   const int32_t per = most <= 2048 ? 1 : most <= 8192 ? 4 : kF8Page;
   const int64_t waves = ceil_div(num_tokens, per) * num_kv_heads;
