@@ -605,7 +605,7 @@ PyObject* prefill_fp8(PyObject* const* a) {
   const int64_t n = q.size(0), hq = q.size(1), start = integer(a[4]);
   int64_t mp;
   const at::Tensor& bt = table_of(a[3], P.dev, mp);
-  need(start >= 0 && start + n <= mp * P.bs);
+  need(start >= 0 && start <= mp * P.bs - n);
   const float scale = scale_of(a[6], P.d);
   const int32_t N = small(n), Q = small(hq);
   const Call w = call_on(a[8], P.dev, E.prefill_fp8_ws(N, int32_t(start), Q, P.hkv, P.d, P.bs));
@@ -636,7 +636,12 @@ PyObject* evict(PyObject* const* a) {
   const uint8_t* act = mask(a[6], dev, n);
   const int32_t bs = small(integer(a[7]));
   at::Tensor t, l, ow, g;
-  unlocked([&] { t = at::empty({n, mp}, bt.options()); l = at::empty({n}, bt.options()); ow = at::empty({n, w.size(1), mp}, w.options()); g = at::empty({n}, bt.options()); });
+  unlocked([&] {
+    t = at::empty({n, mp}, bt.options());
+    l = at::empty({n}, bt.options());
+    ow = at::empty({n, w.size(1), mp}, w.options());
+    g = at::empty({n}, bt.options());
+  });
   launched(launch(E.evict_pages, static_cast<int32_t*>(t.data_ptr()), static_cast<int32_t*>(l.data_ptr()),
                   static_cast<float*>(ow.data_ptr()), static_cast<int32_t*>(g.data_ptr()),
                   static_cast<const int32_t*>(bt.data_ptr()), small(mp), sl, act, static_cast<const float*>(w.data_ptr()),

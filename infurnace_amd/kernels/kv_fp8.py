@@ -5,8 +5,8 @@ docs/architecture.md:242-253, modules src/infurnace/kernels/kv_store.py and page
 0-byte placeholders) over a cache of half the bytes, for a decode that is bound by them.  A layer's
 cache is two tensors:
 
-  * ``kv_pool`` [2, pages, Hkv, 16, D] ``torch.float8_e4m3fn`` (K = 0, V = 1), or all layers' with a
-    leading layer axis;
+  * ``kv_pool`` [2, pages, Hkv, 16, D] ``torch.float8_e4m3fn`` (K = 0, V = 1; or the codes' bytes as uint8),
+    or all layers' with a leading layer axis;
   * ``scales`` [2, pages, Hkv] fp32: one power of two for each block, the 16 tokens of a page and one
     kv head, of K or of V.  A value is its code times its block's scale.
 
@@ -40,8 +40,10 @@ def _check_cache(kv_pool, scales, layer: int, err: type[ValueError]):
     """(one layer's codes [2, P, Hkv, 16, D], its scales [2, P, Hkv], (P, Hkv, D))."""
     if not isinstance(kv_pool, torch.Tensor) or not isinstance(scales, torch.Tensor):
         raise err("kv_pool and scales must be torch tensors")
+    if kv_pool.dtype == torch.uint8:  # (array libraries without the type hold the codes as bytes)
+        kv_pool = kv_pool.view(_F8)
     if kv_pool.dtype != _F8:
-        raise err(f"kv_pool dtype must be float8_e4m3fn, got {kv_pool.dtype}")
+        raise err(f"kv_pool dtype must be float8_e4m3fn (or uint8, the codes' bytes), got {kv_pool.dtype}")
     if scales.dtype != torch.float32:
         raise err(f"scales dtype must be float32, got {scales.dtype}")
     if kv_pool.ndim not in (5, 6):

@@ -202,6 +202,7 @@ class PagedKVRunner:
         # attention weight of each slot's pages, over its decode steps and their layers
         self.page_weights = (torch.zeros((num_slots, num_kv_heads, self.max_pages), device=self.device)
                              if track_page_weights else None)
+        self._weights_event = None  # after the last change of page_weights
         self._evicted: dict[int, int] = {}  # tokens whose K/V were evicted, by slot
         self.pool = BlockPool(num_blocks, block_size)
         self.mgr = KVManager(self.pool, max_pages_per_seq=self.max_pages)
@@ -391,7 +392,9 @@ class PagedKVRunner:
         for st in self._inflight:  # the engine clears slots between steps: no step takes more launches
             self._close(st)
         if self.page_weights is not None:
+            self._weights_wait()
             self.page_weights[slot].zero_()
+            self._weights_changed()
         self._evicted.pop(slot, None)
         owned = self.mgr.blocks(slot)
         freed = self.mgr.free_sequence(slot)
@@ -425,10 +428,12 @@ class PagedKVRunner:
         if not chosen:
             return []
         rows = self._dev(np.asarray(chosen, np.int64))
+        self._weights_wait()
         table, _, weights, gone = evict_pages(self._dev(self._table(chosen)), self._dev(self.mgr.seq_lens(chosen)),
                                               self.page_weights[rows], keep_pages, sink_pages=sink_pages,
                                               recent_pages=recent_pages)
         self.page_weights[rows] = weights
+        self._weights_changed()
         table, gone = table.cpu().numpy(), gone.cpu().numpy()
         freed: list[int] = []
         for i, s in enumerate(chosen):
@@ -461,9 +466,27 @@ class PagedKVRunner:
     def _close(self, step: _Step) -> None:
         """No launch follows in the step: its page weights go to its slots'."""
         if not step.closed and step.weights is not None:
+            self._weights_wait(step.event)
             self.page_weights.index_add_(0, step.weight_slots, step.weights[step.weight_rows])
+            self._weights_changed(step.weights, step.weight_slots, step.weight_rows)
             step.weights = None
         step.closed = True
+
+    def _weights_wait(self, event=None) -> None:
+        """The current stream waits for the page weights' last change, and for ``event`` (a step may run on another
+        stream than the call that closes it)."""
+        for e in (self._weights_event, event):
+            if isinstance(e, torch.cuda.Event):
+                e.wait()
+
+    def _weights_changed(self, *used: torch.Tensor) -> None:
+        """The page weights were changed on the current stream, reading ``used``."""
+        if self.device.type == "cuda":
+            s = torch.cuda.current_stream(self.device)
+            for t in used:
+                t.record_stream(s)
+            self._weights_event = torch.cuda.Event()
+            self._weights_event.record(s)
 
     def _reserve(self, take):
         """Run a page reservation (all or nothing).  When the pool is exhausted while submitted

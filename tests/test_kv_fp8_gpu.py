@@ -5,7 +5,7 @@ import torch
 
 from fp8_util import EMPTY, F8, RefCache, attend, check, gather, random_cache, tables
 from gpu_util import say
-from infurnace_amd.kernels import paged_attention_fp8, store_kv_fp8, store_kv_fp8_and_decode
+from infurnace_amd.kernels import DeviceArray, evict_pages, paged_attention_fp8, store_kv_fp8, store_kv_fp8_and_decode
 
 pytestmark = pytest.mark.gpu
 
@@ -448,3 +448,108 @@ def test_streams_and_graphs(dev):
         for (g, o, o2, pw), (a, w) in zip(graphs, sets):
             assert torch.equal(o, w) and torch.equal(o2, w)
             assert torch.allclose(pw.sum(-1), torch.full((9, 2), 4.0 * (rep + 1), device=dev), rtol=1e-4)
+
+
+def test_graph_of_a_run(dev):
+    """Append of a chunk, prefill with split keys, decode with weights and eviction in one captured graph, replayed
+    between eager calls of other sizes."""
+    say("fp8 graph of a run")
+    gen = torch.Generator().manual_seed(21)
+    hkv, hq, d, n, start = 2, 8, 128, 40, 2000
+    pages = (start + n) // 16 + 1
+    table = torch.randperm(pages, generator=gen).to(torch.int32).to(dev)
+    pos = torch.arange(start, start + n, device=dev)
+    slots = (table[pos // 16] * 16 + pos % 16).int()
+    ref = random_cache(pages, hkv, d, 5)
+    kv, sc = ref.to(dev)
+    q = torch.randn((n, hq, d), generator=gen).half().to(dev)
+    k, v = rows(gen, n, hkv, d).to(dev), rows(gen, n, hkv, d).to(dev)
+    lens = i32([start + n], dev)
+
+    def run(weights):
+        store_kv_fp8(kv, sc, slots, None, k, v)
+        a = paged_attention_fp8(q, kv, sc, table, None, query_start=start)
+        b = paged_attention_fp8(q[-1:], kv, sc, table[None], lens, page_weights=weights)
+        return (a, b, *evict_pages(table[None], lens, weights, 50, sink_pages=2, recent_pages=3))
+
+    want = run(torch.zeros((1, hkv, pages), device=dev))
+    weights = torch.zeros((1, hkv, pages), device=dev)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        weights.zero_()
+        got = run(weights)
+    for _ in range(4):
+        for t in got:
+            t.zero_()
+        g.replay()
+        paged_attention_fp8(q[:7], kv, sc, table, None, query_start=1500)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+        run(torch.zeros((1, hkv, pages), device=dev))
+
+
+def test_carriers(dev):
+    """Arrays that are no torch tensors, the codes as bytes: the same results as with tensors."""
+    say("fp8 carriers")
+
+    def raw(t):
+        names = {torch.float16: "float16", torch.int32: "int32", torch.float32: "float32", torch.uint8: "uint8"}
+        return DeviceArray(t.data_ptr(), t.shape, names[t.dtype], device=t.device.index, owner=t)
+
+    gen = torch.Generator().manual_seed(3)
+    hkv, hq, d, n = 2, 4, 64, 75
+    table, pages = tables(np.random.default_rng(3), [n])
+    slots = i32(table[0][np.arange(n) // 16] * 16 + np.arange(n) % 16, dev)
+    tab, lens = i32(table, dev), i32([n], dev)
+    q = torch.randn((n, hq, d), generator=gen).half().to(dev)
+    k, v = rows(gen, n, hkv, d).to(dev), rows(gen, n, hkv, d).to(dev)
+    results = []
+    for wrap, kind in ((lambda t: t, F8), (raw, torch.uint8), (lambda t: t, torch.uint8)):
+        codes = torch.zeros((2, pages, hkv, 16, d), dtype=torch.uint8, device=dev)
+        scales = torch.full((2, pages, hkv), EMPTY, device=dev)
+        kv, sc = wrap(codes.view(kind)), wrap(scales)
+        w = torch.zeros((1, hkv, tab.shape[1]), device=dev)
+        store_kv_fp8(kv, sc, wrap(slots), None, wrap(k), wrap(v))
+        a = paged_attention_fp8(wrap(q), kv, sc, wrap(tab), None, query_start=0)
+        b = store_kv_fp8_and_decode(wrap(q[-1:]), kv, sc, wrap(tab), wrap(lens), None, wrap(k[-1:]), wrap(v[-1:]),
+                                    page_weights=wrap(w))
+        e = evict_pages(wrap(tab), wrap(lens), wrap(w), 3)
+        results.append((codes, scales, a, b, w, *e))
+    for other in results[1:]:
+        assert all(torch.equal(x, y) for x, y in zip(results[0], other))
+
+
+def test_native_and_python_calls_agree(dev):
+    """The native argument checks and the Python ones lead to the same calls; what the native ones leave to Python."""
+    say("fp8 native calls")
+    gen = torch.Generator().manual_seed(4)
+    hkv, hq, d = 2, 8, 128
+    lens = [33, 700, 0, 16]
+    table, pages = tables(np.random.default_rng(4), lens)
+    ref = random_cache(pages, hkv, d, 4)
+    q = torch.randn((4, hq, d), generator=gen).half().to(dev)
+    k, v = rows(gen, 4, hkv, d).to(dev), rows(gen, 4, hkv, d).to(dev)
+    tab, ln = i32(table, dev), i32(lens, dev)
+    act = torch.tensor([1, 1, 1, 0], dtype=torch.uint8, device=dev)
+    got = []
+    for validate in (False, True):
+        kv, sc = ref.to(dev)
+        w = torch.zeros((4, hkv, tab.shape[1]), device=dev)
+        o = store_kv_fp8_and_decode(q, kv, sc, tab, ln, act, k, v, page_weights=w, validate=validate)
+        p = paged_attention_fp8(q, kv, sc, tab[1], None, query_start=600, validate=validate)
+        store_kv_fp8(kv, sc, i32([0, 1, 2, 3], dev), act, k, v, validate=validate)
+        got.append((o, p, w, kv.view(torch.uint8), sc))
+    assert all(torch.equal(x, y) for x, y in zip(*got))
+    kv, sc = ref.to(dev)
+    for args in ((q[:, ::2], kv, sc, tab, ln), (q, kv.transpose(1, 2), sc, tab, ln), (q, kv, sc[:, :-1], tab, ln),
+                 (q, kv, sc, tab.long(), ln), (q.float(), kv, sc, tab, ln), (q, kv, sc, tab, ln[:3])):
+        with pytest.raises(ValueError):
+            paged_attention_fp8(*args)
+    for start in (-1, 16 * tab.shape[1] - 3, 2 ** 62):
+        with pytest.raises(ValueError):
+            paged_attention_fp8(q, kv, sc, tab[1], None, query_start=start)
+    with pytest.raises(ValueError, match="not a page"):  # a table entry outside the pool
+        paged_attention_fp8(q, kv, sc, torch.where(tab == tab[1, 2], pages, tab), ln, validate=True)
+    sc[0, int(tab[1, 1]), 0] = 0.75
+    with pytest.raises(ValueError, match="powers of two"):
+        paged_attention_fp8(q, kv, sc, tab, ln, validate=True)

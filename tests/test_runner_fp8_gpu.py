@@ -111,6 +111,39 @@ def test_serving_with_eviction(dev):
     run.synchronize()
 
 
+def test_steps_on_other_streams(dev):
+    """Steps on streams of their own, closed, cleared and evicted from another: the same weights and tables."""
+    say("runner fp8 streams")
+    e = Engine(dev, track_page_weights=True)
+    run = e.run
+    side = [torch.cuda.Stream() for _ in range(2)]
+    for i, (s, n) in enumerate(((0, 200), (1, 90))):
+        with torch.cuda.stream(side[i]):
+            e.prefill(s, n)
+    torch.cuda.synchronize()
+    for step in range(4):
+        with torch.cuda.stream(side[step % 2]):
+            e.decode([0, 1])
+    run.evict(6, recent_pages=2)
+    assert len(run.mgr.blocks(0)) == 6 and len(run.mgr.blocks(1)) == 6
+    run.synchronize()
+    for s, had in ((0, 13), (1, 6)):
+        w = e.weights[s, :, :had]
+        if had > 6:
+            assert torch.all(run.page_weights[s, :, 6:] == 0)
+            assert torch.all(run.page_weights[s].cpu().double().sum(-1) < w.sum(-1) + 1e-6)
+        else:
+            assert torch.allclose(run.page_weights[s, :, :had].cpu().double(), w, rtol=1e-4, atol=1e-6)
+    e.weights = run.page_weights.cpu().double()
+    with torch.cuda.stream(side[0]):
+        e.decode([0, 1])
+    run.clear_slot(1)
+    torch.cuda.synchronize()
+    assert not run.page_weights[1].any()
+    assert torch.allclose(run.page_weights[0].cpu().double(), e.weights[0], rtol=1e-4, atol=1e-6)
+    e.caches_agree()
+
+
 def test_prefix_sharing_and_eviction(dev):
     """An evicted shared page stays the prefix cache's; an evicted slot publishes nothing."""
     say("runner fp8 prefix")
