@@ -675,6 +675,13 @@ static size_t f8_ws_layout(int64_t batch, int64_t wgs, int32_t hkv, int32_t G, i
   return off;
 }
 
+// LDS of a workgroup beside the kernel's own variables (under 2 KB): its states, the rows' offsets, its page sums.
+static size_t f8_lds(int64_t batch, int32_t G, int32_t d, bool weights) {
+  return size_t(2 * kDecWaves) * G * d * sizeof(float) + size_t(batch + 1) * sizeof(int) +
+         (weights ? size_t(kDecWaves) * kWave * G * sizeof(float) : 0);
+}
+constexpr size_t kF8MaxLds = (160 - 2) << 10;
+
 static int f8_decode(void* out, const void* query, void* codes, float* scales, int64_t num_pages,
                      const int32_t* block_tables, int32_t max_pages, const int32_t* seq_lens,
                      const uint8_t* active, const void* new_k, const void* new_v, bool append, float* page_weights,
@@ -689,7 +696,8 @@ static int f8_decode(void* out, const void* query, void* codes, float* scales, i
   const int32_t G = hq / hkv;
   if (block_size != kF8Page || (d != 64 && d != 128 && d != 256) || G > kF8MaxGroup || batch > kF8MaxBatch ||
       int64_t(batch) * hkv > kMaxTickets || max_pages > (1 << 27) / kF8Page ||
-      int64_t(batch) * (max_pages + kRowStart) > (int64_t(1) << 30) || num_pages > (int64_t(1) << 31) / kF8Page)
+      int64_t(batch) * (max_pages + kRowStart) > (int64_t(1) << 30) || num_pages > (int64_t(1) << 31) / kF8Page ||
+      f8_lds(batch, G, d, page_weights != nullptr) > kF8MaxLds)
     return IFN_ERR_UNSUPPORTED;
   IFN_CHECK_ALIGN16(out);
   IFN_CHECK_ALIGN16(query);
@@ -716,8 +724,7 @@ static int f8_decode(void* out, const void* query, void* codes, float* scales, i
   const F8Append ap{static_cast<const f16*>(new_k), static_cast<const f16*>(new_v)};
   const float sl = (scale > 0.f ? scale : 1.f / sqrtf(float(d))) * kLog2e;
   const int64_t blocks = streams / kDecWaves * hkv;
-  const size_t lds = size_t(2 * kDecWaves) * G * d * sizeof(float) + size_t(batch + 1) * sizeof(int) +
-                     (page_weights != nullptr ? size_t(kDecWaves) * kWave * G * sizeof(float) : 0);
+  const size_t lds = f8_lds(batch, G, d, page_weights != nullptr);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   auto launch = [&](auto k) {
     k<<<dim3(unsigned(blocks)), dim3(kDecThreads), lds, s>>>(

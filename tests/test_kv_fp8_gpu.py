@@ -227,6 +227,25 @@ def test_decode_splits(dev, batch, n):
     assert torch.equal(got, again)
 
 
+@pytest.mark.parametrize("batch,d,weights", [(6, 256, True), (2500, 256, True), (4096, 256, False), (4096, 128, True)])
+def test_decode_largest_groups(dev, batch, d, weights):
+    """16 query heads on one kv head and many rows: the most shared memory a call takes."""
+    say(f"decode fp8 largest groups batch={batch} d={d} weights={weights}")
+    rng = np.random.default_rng(batch)
+    lens = rng.integers(0, 40, batch)
+    lens[:3] = [1000, 0, 333]
+    table, pages = tables(rng, lens)
+    ref = random_cache(pages, 1, d, batch)
+    kv, sc = ref.to(dev)
+    q = torch.randn((batch, 16, d), generator=torch.Generator().manual_seed(batch)).half()
+    out, tol, w, wt = ref_decode(ref, table, lens, q)
+    pw = torch.zeros(w.shape, device=dev) if weights else None
+    got = paged_attention_fp8(q.to(dev), kv, sc, i32(table, dev), i32(lens, dev), page_weights=pw)
+    check(got, out, tol, "out")
+    if weights:
+        check(pw, w, w * wt + 1e-30, "weights")
+
+
 def test_decode_masks_caps_and_strange_pages(dev):
     """Inactive rows keep their output; lengths are capped; ids outside the pool hold no keys; a row with no key is
     zero; what lies behind a row's end (NaN codes, any scale) is not seen."""

@@ -49,6 +49,9 @@ def test_decode_entry_points(append):
         assert call(**kw) == _capi.IFN_ERR_INVALID_ARGUMENT
     for kw in (dict(d=96), dict(bs=32), dict(hq=17, hkv=1), dict(B=5000), dict(B=4096, hq=32, hkv=32)):
         assert call(**kw) == _capi.IFN_ERR_UNSUPPORTED
+    # (states, offsets and page sums that shared memory does not hold)
+    assert call(B=4096, hq=16, hkv=1, d=256, pw=A) == _capi.IFN_ERR_UNSUPPORTED
+    assert call(B=4096, hq=16, hkv=1, d=256) == _capi.IFN_ERR_WORKSPACE
     for name in ("out", "q", "c") + (("k", "v") if append else ()):
         assert call(**{name: A + 8}) == _capi.IFN_ERR_ALIGNMENT
     assert call(B=0) == _capi.IFN_OK
