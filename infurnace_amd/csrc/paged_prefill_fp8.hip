@@ -13,9 +13,9 @@
 // registers, as in paged_decode_fp8.hip: K as loaded, V after a byte transpose.  Every 32 columns read and convert a
 // tile again, so calls that fill the chip in workgroups of 128 columns go to paged_prefill_fp8_block.hip.
 //
-// What bounds it: vector work and the L2 (8 KB a tile of 32 x 32), about 0.9 us a tile and SIMD whether it has one
-// wave or two.  512 queries at 1024, 16 / 8 heads x 128 (5.4 GFLOP): 15.7 us, of which 3 before the first tile and 3.5
-// to merge; 16 queries at 4096: 13.3 us.
+// What bounds it: vector work (42% of the waves' time) and waits for loads (33%; 8 KB a tile of 32 x 32, the data path
+// of the L1 76% busy), about 0.9 us a tile and SIMD whether it has one wave or two.  512 queries at 1024, 16 / 8 heads
+// x 128 (5.4 GFLOP): 15.9 us, of which 3 before the first tile and 2 to merge; 16 queries at 4096: 13.3 us.
 #include <algorithm>
 
 #include "kv_fp8.hpp"
