@@ -117,6 +117,17 @@ def _validate_scales(scales: torch.Tensor, table: torch.Tensor, keys: torch.Tens
         raise PagedAttentionError("scales of pages that are read must be positive powers of two")
 
 
+def _validate_append(table: torch.Tensor, keys: torch.Tensor, stores: torch.Tensor, num_pages: int) -> None:
+    """Validate mode: the page that a row's new token goes to (rows with ``stores``) is read by no other row."""
+    need = (keys + BLOCK - 1) // BLOCK
+    used = torch.arange(table.shape[1], device=table.device)[None, :] < need[:, None]
+    times = torch.bincount(table[used].long(), minlength=num_pages)
+    live = (need > 0) & stores
+    last = table[live].gather(1, need[live][:, None] - 1).long()
+    if bool((times[last] != 1).any()):
+        raise PagedAttentionError("the last page of a row is in another row's table: its new token cannot be appended here")
+
+
 def store_kv_fp8(kv_pool: torch.Tensor, scales: torch.Tensor, slot_mapping: torch.Tensor,
                  active_mask: torch.Tensor | None, new_k: torch.Tensor, new_v: torch.Tensor, *, layer: int = 0,
                  validate: bool = False) -> None:
@@ -200,6 +211,8 @@ def _decode(query, kv_pool, scales, block_tables, sequence_lengths, active_mask,
         keys = _row_keys(sequence_lengths, active_mask, msl)
         _validate_pages(block_tables, keys, P, BLOCK, "paged_attention_fp8")
         _validate_scales(scales_layer, block_tables, keys)
+        if append:
+            _validate_append(block_tables, keys, sequence_lengths <= msl, P)
     with _current(dev):
         stream = current_stream(dev)
         nbytes = _capi.lib().ifn_paged_decode_fp8_workspace_bytes(n, hq, hkv, d, BLOCK, max_pages, msl,
@@ -311,7 +324,7 @@ def store_kv_fp8_and_decode(query: torch.Tensor, kv_pool: torch.Tensor, scales: 
     Row b's ``new_k`` / ``new_v`` [B, Hkv, D] fp16 are stored at position ``sequence_lengths[b] - 1`` of its table:
     the same cache and output as ``store_kv_fp8`` of those slots followed by ``paged_attention_fp8``.  Rows that
     are inactive, empty or longer than ``max_seq_len`` store nothing.  A row's last page must be in no other
-    row's table (true of any paged KV state).
+    row's table (true of any paged KV state; ``validate=True`` checks it).
     """
     if not validate and new_k is not None:
         o = _fast.decode_fp8(query, kv_pool, scales, block_tables, sequence_lengths, active_mask, new_k, new_v, layer,

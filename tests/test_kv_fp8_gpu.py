@@ -569,6 +569,12 @@ def test_native_and_python_calls_agree(dev):
             paged_attention_fp8(q, kv, sc, tab[1], None, query_start=start)
     with pytest.raises(ValueError, match="not a page"):  # a table entry outside the pool
         paged_attention_fp8(q, kv, sc, torch.where(tab == tab[1, 2], pages, tab), ln, validate=True)
+    shared = tab.clone()
+    shared[3, 0] = tab[0, 2]  # row 0's last page, where its token goes, is read by row 3
+    store_kv_fp8_and_decode(q, kv, sc, shared, ln, act, k, v, validate=True)  # (row 3 is inactive)
+    with pytest.raises(ValueError, match="another row's table"):
+        store_kv_fp8_and_decode(q, kv, sc, shared, ln, None, k, v, validate=True)
+    paged_attention_fp8(q, kv, sc, shared, ln, validate=True)
     sc[0, int(tab[1, 1]), 0] = 0.75
     with pytest.raises(ValueError, match="powers of two"):
         paged_attention_fp8(q, kv, sc, tab, ln, validate=True)
